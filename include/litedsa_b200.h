@@ -447,6 +447,55 @@ int litedsa_topk_select(const float* logits, const int32_t* lengths, int32_t* to
 /* Status block of the index-logits kernel; same layout and return rule as litedsa_attn_status. */
 int litedsa_index_status(int* out4_host, int reset);
 
+/*
+ * The dense side of latent attention: writing the cache, and attending to all of it.  The reference has no counterpart
+ * of these; they use its cache rows (kernels/b200/dsa/litedsa.cu:82-92 for their widths).
+ *
+ * Appending T tokens to a paged cache, with the rotation by their position applied to the 64 rope dims:
+ *   kv_c      [T, 512] bf16, kv_c_stride elements between tokens (like all strides here a multiple of 8, but
+ *             cos_sin_stride: of 4; bases 16-byte aligned)
+ *   k_rope    [T, 64] bf16
+ *   positions [T] int32, or int64 if positions_64
+ *   cos_sin   [n_positions, 64] fp32: the cosines of a position's 32 angles, then their sines
+ *   slots     [T] int32 or int64: row of the cache, block slots / block_size; no row twice in a call
+ *   cache     [n_blocks, block_size, 576] bf16, or with `packed` 656-byte rows (512 e4m3 codes, 4 fp32 scales, 64 bf16);
+ *             blocks block_stride_bytes apart (a multiple of 16), rows dense
+ *   interleaved: pairs (2i, 2i + 1) of dims are turned, else pairs (i, i + 32)
+ *   q_rope    [T, heads, 64] bf16 -> q_out, turned the same way (may be the same memory), or both NULL
+ *   k_out     [T, 64] bf16: the turned k_rope once more, or NULL
+ * A packed group's scale is the smallest power of two that brings its 128 dims into +-448 (at least 2^-126).  A token whose
+ * slot is negative or beyond the cache has no row written (padding); one whose position is not in the table is left out altogether.
+ */
+int litedsa_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_rope, int64_t k_rope_stride,
+                      const void* positions, int positions_64, const float* cos_sin, int64_t n_positions,
+                      int64_t cos_sin_stride, const void* slots, int slots_64, void* cache, int packed,
+                      int64_t n_blocks, int block_size, int64_t block_stride_bytes, int interleaved,
+                      const void* q_rope, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                      int64_t q_out_token_stride, int64_t q_out_head_stride, int heads, void* k_out,
+                      int64_t k_out_stride, int T, void* stream);
+
+/*
+ * Absorbed latent attention of the last q_len tokens of B sequences over a paged cache:
+ *   out = softmax(sm_scale q . k) k[0:512] over the keys a token sees, lse in natural-log units.
+ *   q           [B, q_len, heads, 576] bf16 (strides in elements, multiples of 8), heads <= 128
+ *   cache       as litedsa_append_kv writes it; block_size a multiple of 16.  A packed row's scales may be any; its values
+ *               are rounded to bf16 (exact for powers of two)
+ *   block_table [B, table_cols] int32, rows table_stride elements apart: block of keys [i block_size, (i + 1) block_size)
+ *   seq_lens    [B] int32: keys of a sequence, its q_len tokens among them; token j sees keys [0, len - q_len + 1 + j).
+ *               Lengths are clamped to [0, table_cols * block_size]; blocks outside the cache read as zeros
+ *   out         [B, q_len, heads, 512] bf16, lse [B, q_len, heads] fp32, dense
+ *   workspace   litedsa_mla_decode_workspace(q_len, heads) bytes on the current device, 16-byte aligned; it holds nothing between calls
+ * A row that sees no key gets out = 0, lse = +inf.  Keys behind a sequence's end are in no result, whatever their rows hold.
+ */
+int64_t litedsa_mla_decode_workspace(int q_len, int heads);
+int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* cache, int packed, int64_t n_blocks, int block_size, int64_t block_stride_bytes,
+                       const int32_t* block_table, int64_t table_stride, int table_cols, const int32_t* seq_lens,
+                       float sm_scale, void* out, float* lse, int B, int q_len, int heads, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+/* Status block of the kernel; same layout and return rule as litedsa_attn_status. */
+int litedsa_mla_decode_status(int* out4_host, int reset);
+
 #ifdef __cplusplus
 }
 #endif

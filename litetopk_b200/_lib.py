@@ -81,6 +81,14 @@ SIGNATURES = {
     "litedsa_topk_select": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64,
                                     c_void_p]),
     "litedsa_index_status": (c_int, [c_void_p, c_int]),
+    "litedsa_append_kv": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                  c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int64, c_int, c_void_p, c_int64,
+                                  c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    "litedsa_mla_decode_workspace": (c_int64, [c_int, c_int]),
+    "litedsa_mla_decode": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int, c_int64,
+                                   c_void_p, c_int64, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int, c_int,
+                                   c_void_p, c_int64, c_void_p]),
+    "litedsa_mla_decode_status": (c_int, [c_void_p, c_int]),
 }
 
 _lib = None

@@ -1,0 +1,741 @@
+// Absorbed latent attention over a paged cache (sm_100a): the decode step of MLA, dense.
+//
+//   s = sm_scale q . k[0:576], p = softmax of s over the keys a row sees, out = p k[0:512]
+//
+// for the rows (token j, head h) of every sequence; token j of q_len sees keys [0, len - q_len + 1 + j).
+// One cache row serves all heads, so a CTA takes up to 64 rows of one sequence and streams its keys once, in blocks of 64:
+//
+//   S   [64 rows x 64 keys]    = Q K^T        (M = 64, N = 64: 36 steps of 16 dims, both operands in shared memory)
+//   O^T [512 dims x R rows]   += V^T P^T      (M = 128 four times, N = R = 16, 32 or 64: A = the K tile itself, read along dims)
+//
+// The second product is taken transposed because O needs 512 columns of tensor memory for 128 lanes of rows, which leaves no
+// room for S, but R columns for each of four times 128 lanes of dims; and because its cost then follows the rows that exist.  The row
+// statistics stay per thread (S has rows on lanes), and only the rare rescaling of O wants them by column, from shared memory.
+//
+// Work is cut along the keys: the blocks of all sequences in a row are dealt to groups of CTAs in equal shares (a group: one
+// CTA per 64 rows of a sequence, which read the same keys at the same time, once from memory and again from L2).  A share's pieces
+// of sequences that other groups have parts of go to a workspace in fp32 and are merged by a second kernel.  Every size but those of the
+// tensors is read on the device, so captured calls follow new lengths.
+//
+// Packed rows (512 e4m3 codes, four fp32 scales, 64 bf16) pass through registers: eight warps load a block ahead, convert it to
+// bf16 (exact where the scales are powers of two) and write the same tile that TMA writes for bf16 rows.
+//
+// A key beyond the sequence's end is in no product: its S is replaced, and its value row is zeroed before the second product, whatever its page holds.
+#include "common.cuh"
+#include "tensor_map.cuh"
+
+namespace lt {
+namespace decode {
+
+constexpr int kD = 576, kDV = 512;
+constexpr int kBlock = 64;                                  // keys
+constexpr int kChunks = kD / 64;
+constexpr uint32_t kChunkBytes = kBlock * 128;              // 64 keys x 64 bf16
+constexpr uint32_t kSlotBytes = kChunks * kChunkBytes;
+constexpr int kSlots = 2;
+constexpr int kWarpMma = 4, kWarpLoad0 = 5, kPackedWarps = 8;
+constexpr int kPackedRow = 656;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kMInit = -1e30f;
+// The running maximum that P is relative to moves only when a row overshoots it by this much (in powers of two): P is at most 2^8,
+// as exact in bf16 as below one, and O is rarely rescaled.
+constexpr float kOvershoot = 8.f;
+
+template <int kRows>
+struct Plan {
+  static constexpr uint32_t kQChunk = kRows * 128;
+  static constexpr uint32_t kOffQ = 0;                      // rows behind kRows that the M = 64 operand covers are whatever lies there
+  static constexpr uint32_t kOffKV = (kChunks * kQChunk + 1023) / 1024 * 1024;
+  static constexpr uint32_t kOffMisc = kOffKV + kSlots * kSlotBytes;
+  static constexpr uint32_t kSmem = kOffMisc + 2048 + 1024;
+  static constexpr uint32_t kTmemS = 4 * kRows;             // columns: O^T, then two S
+  static constexpr uint32_t kTmemCols = 4 * kRows + 128 <= 256 ? 256 : 512;
+  static_assert(kQChunk % 1024 == 0 && (kChunks - 1) * kQChunk + 64 * 128 <= kOffMisc, "the operand ends inside");
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct Misc {
+  uint64_t kv_full[kSlots], s_ready[2], p_ready[2], pv_done[kSlots], q_ready, drained;
+  uint32_t left, tmem_base;
+  int start_b, start_k, count, meta_groups;
+  long long start_pos, total;
+  int scan[16];
+  float corr[64];
+};
+static_assert(sizeof(Misc) <= 2048, "Misc");
+
+struct Params {
+  const uint8_t* q;               // [B, q_len, heads, 576] bf16, byte pitches
+  long long q_b, q_j, q_h;
+  const uint8_t* cache;           // packed rows
+  long long block_pitch;
+  const int32_t* table;           // [B, cols]
+  long long table_pitch;
+  const int32_t* lens;
+  uint8_t* out;                   // [B, rows, 512] bf16
+  float* lse;                     // [B, rows]
+  float* part_o;                  // [CTA][2][kRows][512]
+  float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
+  int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
+  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows;
+  float scale_log2;
+  int epoch;
+  uint32_t wait_limit;
+};
+
+enum { kSiteKv = 1, kSiteS, kSiteP, kSitePv, kSiteQ, kSiteFree };
+static __device__ int g_status[8];
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool softmax_any(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ int len_of(const Params& p, int b) {
+  return (int)min((long long)max(__ldcg(p.lens + b), 0), (long long)p.cols * p.block_size);
+}
+__device__ __forceinline__ int blocks_of(int len) { return max((len + kBlock - 1) / kBlock, 1); }      // an empty sequence: one masked block
+
+// Walks a CTA's share: blocks [k0, k1) of sequence b, piece by piece.
+struct Walk {
+  int b, k0, k1, nb, len, left, index;
+  __device__ __forceinline__ Walk(const Misc& ms) : b(ms.start_b - 1), k0(0), k1(ms.start_k), nb(0), len(0), left(ms.count), index(-1) {}
+  __device__ __forceinline__ bool next(const Params& p) {
+    if (left <= 0) return false;
+    k0 = index < 0 ? k1 : 0;
+    ++b; ++index;
+    len = len_of(p, b);
+    nb = blocks_of(len);
+    k1 = min(nb, k0 + left);
+    left -= k1 - k0;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nb; }
+};
+
+// 16 e4m3 codes x scale -> 16 bf16
+__device__ __forceinline__ void convert16(const uint4& c, float scale, uint4& a, uint4& b) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> (16 * k)), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      o[2 * i + k] = bf16x2(f.x * scale, f.y * scale);
+    }
+  }
+  a = make_uint4(o[0], o[1], o[2], o[3]);
+  b = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
+template <int kRows, bool kPacked>
+__global__ void __launch_bounds__(kPacked ? 32 * (kWarpLoad0 + kPackedWarps) : 32 * (kWarpLoad0 + 1), 1)
+mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
+  using PL = Plan<kRows>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 1023u) & ~1023u;      // swizzled tiles
+  uint8_t* sm = smem_raw + (sbase - raw);
+  Misc& ms = *reinterpret_cast<Misc*>(sm + PL::kOffMisc);
+  const BlockWaiter wt{&ms.left, p.wait_limit};
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int g = (int)blockIdx.x / p.row_tiles, rt = (int)blockIdx.x - g * p.row_tiles;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) { mbar_init(&ms.kv_full[i], kPacked ? kPackedWarps : 1); mbar_init(&ms.pv_done[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4); }
+    mbar_init(&ms.q_ready, 4);
+    mbar_init(&ms.drained, 1);
+    ms.left = 0;
+    ms.count = 0;
+    fence_mbar_init();
+    if (!kPacked) tma_prefetch_desc(&map_kv);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc_cta(&ms.tmem_base, PL::kTmemCols);
+    tmem_relinquish_cta();
+  }
+  pdl_wait();
+  // This group's share: blocks [g total / groups, (g + 1) total / groups) of all sequences' in a row.
+  {
+    const int nt = (int)blockDim.x, per = (p.B + nt - 1) / nt;
+    const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) mine += blocks_of(len_of(p, b));
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    if (lane == 31) ms.scan[warp] = incl;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int before = incl - mine, total = 0;
+    for (int w = 0; w < nt / 32; ++w) {
+      if (w < warp) before += ms.scan[w];
+      total += ms.scan[w];
+    }
+    const int used = min(p.groups, total);
+    const int first = g < used ? (int)((long long)g * total / used) : total, last = g < used ? (int)((long long)(g + 1) * total / used) : total;
+    if (first >= before && first < before + mine && last > first) {
+      int at = before, b = b0;
+      for (;; ++b) {
+        const int nb = blocks_of(len_of(p, b));
+        if (first < at + nb) break;
+        at += nb;
+      }
+      ms.start_b = b; ms.start_k = first - at; ms.count = last - first;
+      ms.start_pos = first; ms.total = total; ms.meta_groups = used;
+    }
+    __syncthreads();
+  }
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem_base, 0);
+
+  if (warp < 4) {
+    // ------------------------------------------------------------ softmax, queries, epilogue
+    // A warp has 16 rows: lane l rows l / 4 and l / 4 + 8, of every 8 keys the pair 2 (l % 4).
+    const int r0 = 16 * warp + (lane >> 2), qd = lane & 3;
+    const bool live = 16 * warp < kRows;
+    const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
+    auto request_q = [&](int b) {
+      for (int i = (int)threadIdx.x; i < kRows * (kD / 8); i += 128) {
+        const int r = i / (kD / 8), c = i - r * (kD / 8), row = rt * kRows + r;
+        const uint32_t dst = sbase + PL::kOffQ + (uint32_t)(c >> 3) * PL::kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        const int j = row / p.heads, h = row - j * p.heads;
+        const bool in = row < p.rows;
+        cp_async16_or_zero(dst, p.q + (in ? b * p.q_b + j * p.q_j + h * p.q_h + 16 * c : 0), in);
+      }
+    };
+    auto pass_q = [&]() {
+      cp_async_wait_all();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ms.q_ready);
+    };
+    Walk w(ms);
+    int kb = 0;
+    // A wait here that gives up is passed like any other: the four warps meet at named barriers, so they take the same steps.
+    bool more = w.next(p);
+    if (more) { request_q(w.b); pass_q(); }
+    while (more) {
+      // rows' limits
+      int lim[2], low;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = rt * kRows + r0 + 8 * i;
+        lim[i] = min(w.len, w.len - p.q_len + 1 + row / p.heads);
+      }
+      low = w.len - p.q_len + 1 + rt * kRows / p.heads;                   // what the tile's first row sees
+      float m[2] = {kMInit, kMInit}, l[2] = {0.f, 0.f};
+      Walk ahead = w;
+      const bool another = ahead.next(p);
+      for (int k = w.k0; k < w.k1; ++k, ++kb) {
+        mbar_wait(&ms.s_ready[kb & 1], (kb >> 1) & 1, wt, kSiteS, kb);
+        tc_fence_after();
+        if (k + 1 == w.k1 && another) request_q(ahead.b);                 // all products with this piece's Q are complete
+        float v[2][16];
+        float mx[2] = {-INFINITY, -INFINITY};
+        if (live) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tmem_ld_16x256b_x4(tmem + PL::kTmemS + 64 * (kb & 1) + 32 * c + lane_base, v[c]);
+          tmem_wait_ld();
+          const int key0 = k * kBlock + 2 * qd;
+          if ((k + 1) * kBlock > low) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int key = key0 + 32 * c + 8 * (e >> 2) + (e & 1);
+                v[c][e] = key < lim[(e >> 1) & 1] ? v[c][e] * p.scale_log2 : -INFINITY;
+              }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[c][e] *= p.scale_log2;
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], v[c][e]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+          }
+        }
+        if (k == w.k0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) m[i] = fmaxf(m[i], mx[i]);
+        } else if (softmax_any(mx[0] > m[0] + kOvershoot || mx[1] > m[1] + kOvershoot)) {
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float now = fmaxf(m[i], mx[i]), f = fast_exp2(m[i] - now);
+              m[i] = now;
+              l[i] *= f;
+              if (qd == 0) ms.corr[r0 + 8 * i] = f;
+            }
+          }
+          softmax_sync();
+          mbar_wait(&ms.pv_done[(kb - 1) & 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 4 * kRows; c += 16) {
+            float o[16];
+            tmem_ld16(tmem + lane_base + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] *= ms.corr[(c & (kRows - 1)) + e];
+            const uint32_t* r = reinterpret_cast<const uint32_t*>(o);
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                         ::"r"(tmem + lane_base + c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+          }
+          tmem_wait_st();
+        }
+        const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+        if (live) {
+          // P takes the place of the block's rope dims, which the first product was the last to read
+          const uint32_t prow = slot + (kChunks - 1) * kChunkBytes + r0 * 128 + 4 * qd;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float e[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                e[x] = fast_exp2(v[c][4 * i + x] - m[x >> 1]);
+                l[x >> 1] += e[x];
+              }
+              const uint32_t at = prow + (((4 * c + i) ^ (r0 & 7)) << 4);
+              st_shared4(at, bf16x2(e[0], e[1]));
+              st_shared4(at + 8 * 128, bf16x2(e[2], e[3]));
+            }
+        }
+        const int valid = w.len - k * kBlock;
+        if (valid < kBlock) {                                             // value rows behind the end: nothing, whatever the page holds
+          const int from = max(valid, 0);
+          for (int i = (int)threadIdx.x; i < (kBlock - from) * 64; i += 128)
+            st_shared16(slot + (uint32_t)((i >> 3) & 7) * kChunkBytes + (from + (i >> 6)) * 128 + (i & 7) * 16, make_uint4(0, 0, 0, 0));
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.p_ready[kb & 1]);
+      }
+      if (another) pass_q();
+      // epilogue: O^T has dims on lanes; a warp writes 32 dims of a row at a time
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      }
+      const bool whole = w.whole();
+      const int slot = (int)blockIdx.x * 2 + (w.index == 0 ? 0 : 1);
+      softmax_sync();                                                     // corr of an earlier rescaling has been read
+      if (live && qd == 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = r0 + 8 * i, row = rt * kRows + r;
+          ms.corr[r] = whole ? (l[i] > 0.f ? 1.f / l[i] : 0.f) : 1.f;
+          if (whole) {
+            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = l[i] > 0.f ? (m[i] + __log2f(l[i])) * kLn2 : INFINITY;
+          } else {
+            p.part_ml[(long long)slot * kRows + r] = make_float2(m[i], l[i]);
+          }
+        }
+      softmax_sync();
+      mbar_wait(&ms.pv_done[(kb - 1) & 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+      tc_fence_after();
+      const int rows = min(kRows, p.rows - rt * kRows);
+#pragma unroll 1
+      for (int c = 0; c < 4 * kRows; c += 16) {
+        float o[16];
+        tmem_ld16(tmem + lane_base + c, o);
+        tmem_wait_ld();
+        const int r = c & (kRows - 1), d = c / kRows * 128 + 32 * warp + lane;
+        if (whole) {
+          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kRows + r) * kDV + d;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (r + e < rows) {
+              const float f = ms.corr[r + e];
+              dst[e * kDV] = __float2bfloat16(f > 0.f ? o[e] * f : 0.f);      // a row without keys: 0, whatever the values of others
+            }
+        } else {
+          float* dst = p.part_o + ((long long)slot * kRows + r) * kDV + d;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (r + e < rows) dst[e * kDV] = o[e];
+        }
+      }
+      tc_fence_before();
+      w = ahead;
+      more = another;
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------------------ the two products (one thread)
+    if (elect_one()) {
+      constexpr uint32_t idesc_qk = umma_idesc(1, 1, false, false, 64, kBlock);
+      constexpr uint32_t idesc_pv = umma_idesc(1, 1, true, false, 128, kRows);
+      const uint64_t q_desc = umma_desc(sbase + PL::kOffQ, 16, 1024, kSwz128);
+      bool ok = true;
+      auto qk = [&](int kb) {
+        if (!(ok = mbar_wait(&ms.kv_full[kb & 1], (kb >> 1) & 1, wt, kSiteKv, kb))) return;
+        tc_fence_after();
+        const uint64_t kd = umma_desc(sbase + PL::kOffKV + (kb & 1) * kSlotBytes, 16, 1024, kSwz128);
+        const uint32_t d = tmem + PL::kTmemS + 64 * (kb & 1);
+#pragma unroll 1
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            mma_f16(d, q_desc + (PL::kQChunk >> 4) * j + 2 * s, kd + (kChunkBytes >> 4) * j + 2 * s, idesc_qk, (uint32_t)(j | s));
+        mma_commit_cta(&ms.s_ready[kb & 1]);
+      };
+      auto pv = [&](int kb, bool first) {
+        if (!(ok = mbar_wait(&ms.p_ready[kb & 1], (kb >> 1) & 1, wt, kSiteP, kb))) return;
+        tc_fence_after();
+        const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+        const uint64_t vd = umma_desc(slot, kChunkBytes, 1024, kSwz128);                            // dims along M: two chunks of 64, 8 keys 1024 bytes
+        const uint64_t pd = umma_desc(slot + (kChunks - 1) * kChunkBytes, 16, 1024, kSwz128);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            mma_f16(tmem + kRows * i, vd + (2 * kChunkBytes >> 4) * i + 128 * s, pd + 2 * s, idesc_pv, first && s == 0 ? 0u : 1u);
+        mma_commit_cta(&ms.pv_done[kb & 1]);
+      };
+      Walk w(ms);
+      int kb = 0, seg = 0;
+      bool first_before = false;                                          // whether block kb - 1 is its piece's first
+      for (; ok && w.next(p); ++seg) {
+        for (int k = w.k0; ok && k < w.k1; ++k, ++kb) {
+          const bool first = k == w.k0;
+          // the next piece's queries come in while its predecessor's last block is finished
+          if (first) {
+            if (kb > 0) pv(kb - 1, first_before);
+            if (ok) ok = mbar_wait(&ms.q_ready, seg & 1, wt, kSiteQ, kb);
+            if (ok) qk(kb);
+          } else {
+            qk(kb);
+            if (ok) pv(kb - 1, first_before);
+          }
+          first_before = first;
+        }
+      }
+      if (ok && kb > 0) pv(kb - 1, first_before);
+      if (!ok) {                                                          // given up: what has been issued ends before the tensor memory goes
+        mma_commit_cta(&ms.drained);
+        mbar_drain(&ms.drained, 0);
+      }
+    }
+    __syncwarp();
+  } else if (!kPacked) {
+    // ------------------------------------------------------------ bf16 rows by TMA
+    Walk w(ms);
+    int kb = 0, asked = 0;
+    bool ok = true;
+    const int boxes = kBlock / p.box_rows;                                // a box: rows of one page (at most 64), 64 dims
+    while (ok && w.next(p)) {
+      const int32_t* table = p.table + w.b * p.table_pitch;
+      for (int k = w.k0; k < w.k1; ++k, ++kb) {
+        int page = 0;                                                     // lane i: box i's page
+        const int at = k * kBlock + lane * p.box_rows;
+        const bool in = lane < boxes && at < w.len;
+        if (in) page = __ldcg(table + at / p.block_size);
+        const int n = __popc(__ballot_sync(0xffffffffu, in));
+        if (kb >= kSlots && !(ok = mbar_wait(&ms.pv_done[kb & 1], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1], (uint32_t)(n * p.box_rows * kD * 2));
+        __syncwarp();
+        for (int i = 0; i < n; ++i) {
+          const int pg = __shfl_sync(0xffffffffu, page, i), row = (k * kBlock + i * p.box_rows) % p.block_size;
+          if (lane < kChunks)
+            tma_load_3d_hint(sbase + PL::kOffKV + (kb & 1) * kSlotBytes + lane * kChunkBytes + i * p.box_rows * 128, &map_kv, 64 * lane, row, pg,
+                             &ms.kv_full[kb & 1], l2_policy_evict_first());
+        }
+        asked = kb + 1;
+      }
+    }
+    if (!ok)
+      for (int i = max(asked - kSlots, 0); i < asked; ++i) mbar_drain(&ms.kv_full[i & 1], (i >> 1) & 1);
+  } else {
+    // ------------------------------------------------------------ packed rows through registers
+    // Warp v has rows v, v + 8, ..: a lane 16 codes of each, and 16 bytes of two rows' rope dims.
+    const int v = warp - kWarpLoad0;
+    uint4 codes[8], rope[2];
+    float scale[8];
+    auto row_at = [&](const Walk& w, int key) -> const uint8_t* {
+      const int page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
+      if ((unsigned)page >= (unsigned)p.n_blocks) return nullptr;
+      return p.cache + (long long)page * p.block_pitch + (long long)(key % p.block_size) * kPackedRow;
+    };
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto load = [&](const Walk& w, int k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = k * kBlock + v + 8 * i;
+        const uint8_t* src = key < w.len ? row_at(w, key) : nullptr;
+        codes[i] = zero;
+        scale[i] = 0.f;
+        if (src) {
+          codes[i] = __ldcs(reinterpret_cast<const uint4*>(src) + lane);
+          scale[i] = __ldcg(reinterpret_cast<const float*>(src + 512) + (lane >> 3));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = k * kBlock + v + 8 * (4 * i + (lane >> 3));
+        const uint8_t* src = key < w.len ? row_at(w, key) : nullptr;
+        rope[i] = src ? __ldcs(reinterpret_cast<const uint4*>(src + 528) + (lane & 7)) : zero;
+      }
+    };
+    Walk w(ms);
+    bool more = w.next(p);
+    int k = w.k0, kb = 0;
+    if (more) load(w, k);
+    while (more) {
+      if (kb >= kSlots && !mbar_wait(&ms.pv_done[kb & 1], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)) break;
+      const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = v + 8 * i;
+        uint4 a, b;
+        convert16(codes[i], scale[i], a, b);
+        // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
+        const uint32_t base = slot + (uint32_t)(lane >> 2) * kChunkBytes + r * 128;
+        const uint32_t u = 2 * (lane & 3), odd = (lane >> 2) & 1;
+        st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
+        st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = v + 8 * (4 * i + (lane >> 3));
+        st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), rope[i]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1]);
+      ++kb;
+      if (++k == w.k1) {
+        more = w.next(p);
+        k = w.k0;
+      }
+      if (more) load(w, k);
+    }
+  }
+
+  // which sequence of this group others have the rest of
+  if (warp == kWarpMma && rt == 0 && lane == 0 && p.meta) {
+    int4 e = make_int4(-1, 0, 0, 0);
+    Walk w(ms);
+    int before = 0;
+    while (w.next(p)) {
+      if (w.k0 == 0 && w.k1 < w.nb) {
+        const long long end = ms.start_pos + before + w.nb;               // behind the sequence's last block
+        e = make_int4(w.b, w.index == 0 ? 0 : 1, (int)((end * ms.meta_groups - 1) / ms.total) - g + 1, 0);
+      }
+      before += w.k1 - w.k0;
+    }
+    p.meta[g] = e;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma) tmem_dealloc_cta(tmem, PL::kTmemCols);
+  if (threadIdx.x == 0) {
+    wt.report(g_status, p.epoch);
+    if (blockIdx.x == 0) atomicAdd(&g_status[3], 1);
+  }
+}
+
+// The parts of row blockIdx.x of the blockIdx.y-th sequence that several groups have: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
+// A warp sums every eighth part, all loads of four parts under way; the eight sums meet in shared memory.
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(32 * kMergeWarps) mla_decode_merge_kernel(const Params p, int kRows) {
+  __shared__ float4 acc[kMergeWarps][kDV / 4];
+  __shared__ float sum_l[kMergeWarps];
+  __shared__ int pick[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
+  if (warp == 0) {                                   // the blockIdx.y-th entry of the list
+    int seen = 0, found = -1;
+    for (int g0 = 0; g0 < p.groups && found < 0; g0 += 32) {
+      const bool is = g0 + lane < p.groups && __ldcg(&p.meta[g0 + lane].x) >= 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, is);
+      const int want = (int)blockIdx.y - seen;
+      if (want < __popc(mask)) found = g0 + (int)__fns(mask, 0, want + 1);
+      seen += __popc(mask);
+    }
+    if (lane == 0) pick[0] = found;
+  }
+  __syncthreads();
+  const int g = pick[0];
+  if (g < 0) return;
+  const int4 e = __ldcg(p.meta + g);
+  const int row = (int)blockIdx.x, rt = row / kRows, r = row - rt * kRows, parts = e.z;
+  auto slot_of = [&](int i) -> long long { return ((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r; };
+  float m = kMInit;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(&p.part_ml[slot_of(i)].x));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float4 a[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i0 = warp; i0 < parts; i0 += 4 * kMergeWarps) {
+    float4 v[4][4];
+    float2 ml[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kMergeWarps;
+      ml[u] = make_float2(kMInit, 0.f);
+      if (i < parts) {
+        const long long s = slot_of(i);
+        ml[u] = __ldcg(&p.part_ml[s]);
+        const float4* src = reinterpret_cast<const float4*>(p.part_o + s * kDV);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[u][c] = __ldcg(src + 32 * c + lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!(ml[u].y > 0.f)) continue;                // beyond the list, or a part without keys
+      const float f = fast_exp2(ml[u].x - m);
+      l += f * ml[u].y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        a[c].x += f * v[u][c].x; a[c].y += f * v[u][c].y; a[c].z += f * v[u][c].z; a[c].w += f * v[u][c].w;
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc[warp][32 * c + lane] = a[c];
+  if (lane == 0) sum_l[warp] = l;
+  __syncthreads();
+  if (threadIdx.x >= kDV / 4) return;
+  float4 o = acc[0][threadIdx.x];
+  l = sum_l[0];
+#pragma unroll
+  for (int w = 1; w < kMergeWarps; ++w) {
+    const float4 x = acc[w][threadIdx.x];
+    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    l += sum_l[w];
+  }
+  const float f = l > 0.f ? 1.f / l : 0.f;
+  const long long at = (long long)e.x * p.rows + row;
+  reinterpret_cast<uint2*>(p.out)[at * (kDV / 4) + threadIdx.x] = make_uint2(bf16x2(o.x * f, o.y * f), bf16x2(o.z * f, o.w * f));      // (all parts without keys: o = 0)
+  if (threadIdx.x == 0) p.lse[at] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+}
+
+static int rows_per_cta(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+struct Shape {
+  int per, tiles, groups;
+  Shape(int rows) {
+    per = rows_per_cta(rows);
+    tiles = (rows + per - 1) / per;
+    groups = max(1, sm_count() / tiles);
+  }
+  int64_t part_bytes() const { return (int64_t)groups * tiles * 2 * per * (kDV * 4 + 8); }
+  int64_t bytes() const { return groups == 1 ? 0 : part_bytes() + (int64_t)groups * 16; }
+};
+
+template <int kRows, bool kPacked>
+static int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
+  if (!ensure_smem<mla_decode_kernel<kRows, kPacked>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
+  return launch_pdl(mla_decode_kernel<kRows, kPacked>, dim3((unsigned)(p.groups * p.row_tiles)), 32 * (kWarpLoad0 + (kPacked ? kPackedWarps : 1)),
+                    Plan<kRows>::kSmem, st, map, p);
+}
+
+}  // namespace decode
+}  // namespace lt
+
+extern "C" int64_t litedsa_mla_decode_workspace(int q_len, int heads) {
+  if (q_len <= 0 || heads <= 0 || heads > 128 || (int64_t)q_len * heads > (1 << 20)) return 0;
+  return lt::decode::Shape(q_len * heads).bytes();
+}
+
+extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                  const void* cache, int packed, int64_t n_blocks, int block_size, int64_t block_stride_bytes,
+                                  const int32_t* block_table, int64_t table_stride, int table_cols, const int32_t* seq_lens,
+                                  float sm_scale, void* out, float* lse, int B, int q_len, int heads, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  using namespace lt;
+  using namespace lt::decode;
+  if (!q || (!cache && n_blocks > 0) || (!block_table && table_cols > 0) || !seq_lens || !out || !lse) return LITEDSA_ERR_ARG;
+  if (B < 0 || q_len <= 0 || heads <= 0 || heads > 128 || (int64_t)q_len * heads > (1 << 20) || table_cols < 0 || n_blocks < 0 || block_size <= 0)
+    return LITEDSA_ERR_SHAPE;
+  if (block_size % 16 || n_blocks >= (1ll << 31) || (int64_t)table_cols * block_size >= (1ll << 31) - kBlock) return LITEDSA_ERR_UNSUPPORTED;
+  const int row = packed ? kPackedRow : 2 * kD;
+  if (n_blocks > 1 && block_stride_bytes < (int64_t)block_size * row) return LITEDSA_ERR_SHAPE;
+  if (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out | (uintptr_t)workspace) & 15 || block_stride_bytes % 16 ||
+      (q_batch_stride | q_token_stride | q_head_stride) % 8 || ((uintptr_t)lse & 3))
+    return LITEDSA_ERR_UNSUPPORTED;
+  if (B == 0) return LITEDSA_OK;
+  const Shape s(q_len * heads);
+  if (s.bytes() > 0 && (!workspace || workspace_bytes < s.bytes())) return workspace ? LITEDSA_ERR_SHAPE : LITEDSA_ERR_ARG;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  Params p = {};
+  p.q = reinterpret_cast<const uint8_t*>(q);
+  p.q_b = 2 * q_batch_stride; p.q_j = 2 * q_token_stride; p.q_h = 2 * q_head_stride;
+  p.cache = reinterpret_cast<const uint8_t*>(cache); p.block_pitch = block_stride_bytes;
+  p.table = block_table; p.table_pitch = table_stride; p.lens = seq_lens;
+  p.out = reinterpret_cast<uint8_t*>(out); p.lse = lse;
+  if (s.groups > 1) {
+    p.part_o = reinterpret_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)s.groups * s.tiles * 2 * s.per * kDV);
+    p.meta = reinterpret_cast<int4*>(reinterpret_cast<char*>(workspace) + s.part_bytes());
+  }
+  p.B = B; p.q_len = q_len; p.heads = heads; p.rows = q_len * heads; p.row_tiles = s.tiles; p.groups = s.groups;
+  p.cols = n_blocks == 0 ? 0 : table_cols; p.block_size = block_size; p.n_blocks = (int)n_blocks;
+  p.box_rows = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
+  p.scale_log2 = sm_scale * kLog2e;
+  p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
+  CUtensorMap map = {};
+  if (!packed && n_blocks > 0 &&
+      !make_map_3d(&map, cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)block_size, (uint64_t)n_blocks, 2 * kD,
+                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, (uint32_t)p.box_rows, 1))
+    return LITEDSA_ERR_CUDA;
+  int rc;
+  if (s.per == 16) rc = packed ? launch<16, true>(map, p, st) : launch<16, false>(map, p, st);
+  else if (s.per == 32) rc = packed ? launch<32, true>(map, p, st) : launch<32, false>(map, p, st);
+  else rc = packed ? launch<64, true>(map, p, st) : launch<64, false>(map, p, st);
+  if (rc != LITEDSA_OK || s.groups == 1) return rc;
+  return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)p.rows, (unsigned)min(B, s.groups)), 32 * kMergeWarps, 0, st, p, s.per);
+}
+
+// Status block of the kernel; layout and return rule as litedsa_attn_status.
+extern "C" int litedsa_mla_decode_status(int* out4_host, int reset) {
+  using namespace lt::decode;
+  if (out4_host && cudaMemcpyFromSymbol(out4_host, g_status, sizeof(int) * 4) != cudaSuccess) return LITEDSA_ERR_CUDA;
+  if (reset) {
+    const int z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (cudaMemcpyToSymbol(g_status, z, sizeof(z)) != cudaSuccess) return LITEDSA_ERR_CUDA;
+  }
+  return (out4_host && out4_host[0] != 0) ? LITEDSA_ERR_TIMEOUT : LITEDSA_OK;
+}
