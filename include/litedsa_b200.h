@@ -485,7 +485,8 @@ int litedsa_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_rope,
  *               Lengths are clamped to [0, table_cols * block_size]; blocks outside the cache read as zeros
  *   out         [B, q_len, heads, 512] bf16, lse [B, q_len, heads] fp32, dense
  *   workspace   litedsa_mla_decode_workspace(q_len, heads) bytes on the current device, 16-byte aligned; it holds nothing between calls
- * A row that sees no key gets out = 0, lse = +inf.  Keys behind a sequence's end are in no result, whatever their rows hold.
+ * A row that sees no key gets out = 0, lse = +inf.  Keys behind a sequence's end are in no result, whatever their rows hold; a
+ * value that is infinite or NaN can reach the earlier of the sequence's new tokens, although they may not see it.
  */
 int64_t litedsa_mla_decode_workspace(int q_len, int heads);
 int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -495,6 +496,29 @@ int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_st
                        int64_t workspace_bytes, void* stream);
 /* Status block of the kernel; same layout and return rule as litedsa_attn_status. */
 int litedsa_mla_decode_status(int* out4_host, int reset);
+
+/*
+ * Expanded latent attention of the queries of B sequences over their keys, per head:
+ *   out = softmax(sm_scale (q[0:128] . k_nope + q[128:192] . k_rope)) v, lse in natural-log units.
+ *   q       [Tq, heads, 192] bf16, k_nope [Tk, heads, 128] bf16, k_rope [Tk, 64] bf16 (one for all heads), v [Tk, heads, 128] bf16
+ *           (strides in elements, multiples of 8; bases 16-byte aligned)
+ *   cu_q, cu_k  [B + 1] int32: sequence b has queries [cu_q[b], cu_q[b + 1]) and keys [cu_k[b], cu_k[b + 1]); both NULL
+ *           with B = 1: one sequence of all.  Entries are clamped to [0, Tq] and [0, Tk]; rows of out and lse that are no sequence's stay as they were
+ *   causal  query i of a sequence with n queries and m keys sees keys [0, m - n + 1 + i) (its queries are its last tokens), else all
+ *   out     [Tq, heads, 128] bf16, lse [Tq, heads] fp32, dense
+ *   workspace   litedsa_mla_prefill_workspace(Tq, Tk, heads) bytes (0 for most sizes) on the current device, 16-byte
+ *           aligned; it holds nothing between calls
+ * sm_scale is not negative.  A row that sees no key gets out = 0, lse = +inf.  Keys of other sequences and behind the last one are in no result,
+ * whatever they hold; a value that is infinite or NaN can reach the rows of its sequence that share a block of 128 keys
+ * with it, although they may not see it.
+ */
+int64_t litedsa_mla_prefill_workspace(int Tq, int Tk, int heads);
+int litedsa_mla_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_nope, int64_t k_token_stride,
+                        int64_t k_head_stride, const void* k_rope, int64_t k_rope_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int B, float sm_scale, int causal, void* out,
+                        float* lse, int Tq, int Tk, int heads, void* workspace, int64_t workspace_bytes, void* stream);
+/* Status block of the kernel; same layout and return rule as litedsa_attn_status. */
+int litedsa_mla_prefill_status(int* out4_host, int reset);
 
 #ifdef __cplusplus
 }

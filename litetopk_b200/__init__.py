@@ -9,11 +9,12 @@ from .api import (attn_status, bf16_status, dequant_kv656, dsv4_c128a_bf16,  # n
                   dsv4_masked_mla_bf16_out, dsv4_status, masked_mla_bf16_out, masked_mla_fp8,
                   masked_mla_fp8_out, merge_kv_splits, prepare_kv, quantize_e4m3, repack_kv656, sparse_prefill,
                   sparse_prefill_host, union_qm, union_qm_out)
-from .dense import append_kv, mla_decode, mla_decode_status  # noqa: F401
+from .dense import append_kv, mla_decode, mla_decode_status, mla_prefill, mla_prefill_status  # noqa: F401
 from . import synth  # noqa: F401
 
 __all__ = ["union_qm", "union_qm_out", "masked_mla_fp8", "masked_mla_fp8_out", "masked_mla_bf16_out",
            "dsv4_c128a_bf16", "dsv4_masked_mla_bf16_out", "sparse_prefill", "sparse_prefill_host",
            "prepare_kv", "merge_kv_splits", "quantize_e4m3", "repack_kv656", "dequant_kv656", "attn_status",
            "bf16_status", "dsv4_status", "index_logits_fp8", "topk_select", "lite_topk",
-           "index_status", "append_kv", "mla_decode", "mla_decode_status", "synth"]
+           "index_status", "append_kv", "mla_decode", "mla_decode_status", "mla_prefill",
+           "mla_prefill_status", "synth"]

@@ -89,6 +89,11 @@ SIGNATURES = {
                                    c_void_p, c_int64, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int, c_int,
                                    c_void_p, c_int64, c_void_p]),
     "litedsa_mla_decode_status": (c_int, [c_void_p, c_int]),
+    "litedsa_mla_prefill_workspace": (c_int64, [c_int, c_int, c_int]),
+    "litedsa_mla_prefill": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                    c_int64, c_int64, c_void_p, c_void_p, c_int, c_float, c_int, c_void_p, c_void_p,
+                                    c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
+    "litedsa_mla_prefill_status": (c_int, [c_void_p, c_int]),
 }
 
 _lib = None

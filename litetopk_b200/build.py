@@ -22,7 +22,7 @@ OUT_DIR = PKG / "_C"
 LIB = OUT_DIR / "liblitedsa_b200.so"
 HOST_SRC = CSRC / "host_binding.cpp"
 SOURCES = ["abi.cu", "union_qm.cu", "attn_fp8.cu", "prep.cu", "noalloc.cu", "attn_dsv4.cu", "attn_bf16.cu", "peak_probe.cu", "index_topk.cu",
-           "prefill.cu", "append_kv.cu", "mla_decode.cu"]
+           "prefill.cu", "append_kv.cu", "mla_decode.cu", "mla_prefill.cu"]
 
 
 def _nvcc() -> str:

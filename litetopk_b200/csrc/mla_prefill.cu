@@ -1,0 +1,666 @@
+// Expanded latent attention (sm_100a): the dense prefill of MLA over a batch of sequences of their own lengths.
+//
+//   s = sm_scale (q[0:128] . k_nope + q[128:192] . k_rope), p = softmax of s over the keys a token sees, out = p v[0:128]
+//
+// per head; k_rope is one vector a token for all heads.  Bound by the tensor cores: 640 flops a (query, key, head).
+//
+// A CTA takes 256 queries of a head as two tiles of 128 rows and streams the keys in blocks of 128.  Tensor memory is full: two S
+// (128 columns each; P, bf16, takes the place of its S and is the A operand of the second product from there) and two O.
+// While one tile's S is turned into P by its four warps, the tensor cores have the other tile's products:
+//
+//   P0 V(i), Q0 K(i+1), P1 V(i), Q1 K(i+1), P0 V(i+1), ...
+//
+// A thread has a row: no reductions between threads, and the rare rescaling of O is its warp's own business (the running maximum
+// that P is relative to moves only when a row overshoots it by 2^8).  Keys and values pass through one ring of eight 16 KB
+// granules (128 tokens x 64 dims) in the order of use, three of K and two of V a block: with a stage of K and of V each released as a whole
+// the V of a block would come too late.
+//
+// CTAs take work dynamically (cluster launch control: a running CTA takes the place of one that has not been launched), the heavy
+// tiles of a head first, heads one after the other so that the CTAs that run share their K and V in L2.  A call of few tiles leaves
+// most of its last wave idle: its last tiles are cut along the keys, and a second kernel merges the pieces in fp32.
+#include "common.cuh"
+#include "tensor_map.cuh"
+
+namespace lt {
+namespace prefill {
+
+constexpr int kRows = 128, kPair = 256, kBlock = 128, kDV = 128;
+constexpr uint32_t kGranule = 128 * 128;                    // 128 tokens x 64 bf16
+constexpr int kRing = 8, kPerBlock = 5;                     // granules; of a block: K 0-2, V 3-4
+constexpr uint32_t kQTile = 3 * kGranule;
+constexpr uint32_t kOffQ = 0, kOffRing = 2 * kQTile, kOffMisc = kOffRing + kRing * kGranule;
+constexpr uint32_t kSmem = kOffMisc + 1024 + 1024;
+static_assert(kSmem <= 232448, "shared memory");
+constexpr int kWarpMma = 8, kWarpLoad = 9, kThreads = 384;     // (warps 10 and 11 have nothing to do: registers are dealt out by four warps)
+constexpr uint32_t kTmemO = 256;                            // S0, S1, O0, O1: 128 columns each
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kMInit = -1e30f;
+constexpr float kOvershoot = 8.f;
+
+struct Work {
+  int head, q0, rows;          // queries [q0, q0 + rows) of the call's tokens
+  int k0, nk;                  // keys of the sequence: [k0, k0 + nk) of the call's
+  int lim0;                    // causal: row r sees keys [0, lim0 + r) of the sequence
+  int b0, n[2];                // blocks [b0, b0 + n[t]) for tile t
+  int part;                    // -1: the tiles as a whole; else which piece's place in the workspace
+  int live;                    // 0: no more work
+};
+struct Misc {
+  uint64_t full[kRing], empty[kRing], q_full[2], q_free[2], s_ready[2], p_ready[2], o_done[2], work_full[2], work_empty[2], clc, drained;
+  uint4 clc_answer;
+  Work work[2];
+  uint32_t left, tmem_base;
+  int scan[2 * kThreads / 32];
+};
+static_assert(sizeof(Misc) <= 1024, "Misc");
+
+struct Params {
+  const int32_t *cu_q, *cu_k;  // [B + 1], or null: one sequence
+  uint8_t* out;                // [Tq, heads, 128] bf16
+  float* lse;                  // [Tq, heads]
+  float* part_o;               // [piece][256][128]
+  float2* part_ml;             // [piece][256]: (maximum, sum)
+  int4* plan;                  // (tiles, first tile that is cut, pieces a tile, 0) for the merge
+  int B, Tq, Tk, heads, ctas, causal, max_pieces;
+  float scale_log2;
+  int epoch;
+  uint32_t wait_limit;
+};
+
+enum { kSiteFull = 1, kSiteEmpty, kSiteQ, kSiteQFree, kSiteS, kSiteP, kSiteO, kSiteWork, kSiteWorkEmpty, kSiteClc };
+static __device__ int g_status[8];
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// work stealing among the blocks of this launch: asks for one that has not started (16 bytes of answer on the barrier)
+__device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int clc_block(const uint4* answer) {      // its blockIdx.x, -1 if there is none
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\t"
+      "ld.shared.v2.b64 {a, b}, [%2];\n\tmov.b128 h, {a, b};\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=r"(x) : "r"(smem_u32(answer)) : "memory");
+  return ok ? (int)x : -1;
+}
+
+__device__ __forceinline__ int start_of(const int32_t* cu, int b, int B, int T) {
+  if (cu == nullptr) return b == 0 ? 0 : T;
+  return min(max(__ldcg(cu + b), 0), T);
+}
+__host__ __device__ __forceinline__ int blocks_seen(int keys) { return keys <= 0 ? 0 : (keys - 1) / kBlock + 1; }
+
+// How the call's tiles (pairs of 128 rows, of all heads) are cut: tiles [0, whole) as they are, the others into `pieces` each.
+// Only calls of few tiles: as many waves of whole tiles as there are, the rest cut so that its pieces fill the CTAs, at a cost of
+// three blocks a piece for its set-up and its way through memory.  Evaluated by one warp.
+struct Cut { int whole, pieces; };
+__device__ __forceinline__ Cut cut_of(int tiles, int most_blocks, const Params& p, int lane) {
+  Cut c{tiles, 1};
+  if (p.max_pieces == 0 || tiles > 4 * p.ctas) return c;
+  const int rest = tiles % p.ctas;
+  if (rest == 0) return c;
+  const int most = min(min(p.max_pieces / rest, most_blocks / 2), 1023);
+  uint32_t best = 0xffffffffu;
+  for (int s = lane + 1; s <= most; s += 32) {
+    const uint32_t cost = (uint32_t)((rest * s + p.ctas - 1) / p.ctas) * (uint32_t)((most_blocks + s - 1) / s + (s > 1 ? 3 : 0));
+    best = min(best, min(cost, 0x3fffffu) << 10 | (uint32_t)s);
+  }
+  best = __reduce_min_sync(0xffffffffu, best);
+  if (best != 0xffffffffu && (best & 1023u) > 1) { c.whole = tiles - rest; c.pieces = (int)(best & 1023u); }
+  return c;
+}
+
+// Work number w, by one warp: tiles of a head from its last to its first, then the next head's.
+__device__ __forceinline__ Work work_of(int w, int tiles_a_head, const Cut& c, const Params& p, int lane) {
+  Work k;
+  k.live = 0;
+  if (tiles_a_head <= 0) return k;                         // no sequence has a query
+  const int tile = w < c.whole ? w : c.whole + (w - c.whole) / c.pieces, piece = w < c.whole ? 0 : (w - c.whole) % c.pieces;
+  k.head = tile / tiles_a_head;
+  k.live = k.head < p.heads;
+  if (!k.live) return k;
+  int at = tiles_a_head - 1 - (tile - k.head * tiles_a_head);
+  int q_start = 0, nq = p.Tq, k_start = 0;
+  k.nk = p.Tk;
+  if (p.cu_q) {
+    int b = 0;
+    for (int b0 = 0;; b0 += 32) {                          // (ends: the tiles of all sequences are tiles_a_head)
+      const int mine = b0 + lane, lo = mine < p.B ? start_of(p.cu_q, mine, p.B, p.Tq) : 0, hi = mine < p.B ? start_of(p.cu_q, mine + 1, p.B, p.Tq) : 0;
+      int incl = (max(hi - lo, 0) + kPair - 1) / kPair;
+      const int own = incl;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, at < incl);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = b0 + l;
+        at -= __shfl_sync(0xffffffffu, incl - own, l);
+        q_start = __shfl_sync(0xffffffffu, lo, l);
+        nq = __shfl_sync(0xffffffffu, hi, l) - q_start;
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, incl, 31);
+      if (b0 + 32 >= p.B) { k.live = 0; return k; }
+    }
+    k_start = start_of(p.cu_k, b, p.B, p.Tk);
+    k.nk = max(start_of(p.cu_k, b + 1, p.B, p.Tk) - k_start, 0);
+  }
+  k.q0 = q_start + at * kPair;
+  k.rows = min(kPair, nq - at * kPair);
+  k.k0 = k_start;
+  k.lim0 = k.nk - nq + at * kPair + 1;
+  int nb[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int last = min(k.rows, kRows * (t + 1)) - 1;     // last row of the tile
+    nb[t] = k.rows <= kRows * t ? 0 : blocks_seen(p.causal ? min(k.nk, k.lim0 + last) : k.nk);
+  }
+  k.part = -1;
+  int from = 0, to = max(nb[0], nb[1]);
+  if (w >= c.whole && c.pieces > 1) {
+    k.part = w - c.whole;
+    from = (int)((long long)to * piece / c.pieces);
+    to = (int)((long long)to * (piece + 1) / c.pieces);
+  }
+  k.b0 = from;
+  k.n[0] = max(min(nb[0], to) - from, 0);
+  k.n[1] = max(min(nb[1], to) - from, 0);
+  return k;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_kr,
+                   const __grid_constant__ CUtensorMap map_v, const Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 1023u) & ~1023u;      // swizzled tiles
+  uint8_t* sm = smem_raw + (sbase - raw);
+  Misc& ms = *reinterpret_cast<Misc*>(sm + kOffMisc);
+  const BlockWaiter wt{&ms.left, p.wait_limit};
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) { mbar_init(&ms.full[i], 1); mbar_init(&ms.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ms.q_full[i], 1); mbar_init(&ms.q_free[i], 1); mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4);
+      mbar_init(&ms.o_done[i], 1); mbar_init(&ms.work_full[i], 1); mbar_init(&ms.work_empty[i], 9);
+    }
+    mbar_init(&ms.clc, 1);
+    mbar_init(&ms.drained, 1);
+    ms.left = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_kn); tma_prefetch_desc(&map_kr); tma_prefetch_desc(&map_v);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc_cta(&ms.tmem_base, 512);
+    tmem_relinquish_cta();
+  }
+  pdl_wait();
+  // tiles of a head and the longest tile's blocks
+  int tiles = 0, most = 0;
+  for (int b = (int)threadIdx.x; b < p.B; b += kThreads) {
+    const int nq = max(start_of(p.cu_q, b + 1, p.B, p.Tq) - start_of(p.cu_q, b, p.B, p.Tq), 0);
+    const int nk = max(start_of(p.cu_k, b + 1, p.B, p.Tk) - start_of(p.cu_k, b, p.B, p.Tk), 0);
+    tiles += (nq + kPair - 1) / kPair;
+    if (nq > 0) most = max(most, blocks_seen(nk));
+  }
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) { ms.scan[2 * warp] = tiles; ms.scan[2 * warp + 1] = most; }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  tiles = most = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) { tiles += ms.scan[2 * w]; most = max(most, ms.scan[2 * w + 1]); }
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem_base, 0);
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax of tile t, a row a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");     // 2 x 200 + 104 = 3 x 168, as launched
+    const int t = warp >> 2, r = 32 * (warp & 3) + lane, rr = kRows * t + r;
+    const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_col = tmem + lane_base + 128 * t, o_col = tmem + lane_base + kTmemO + 128 * t;
+    const float c = p.scale_log2;
+    const uint64_t c2 = pack2(c, c);
+    int ns = 0, no = 0, block0 = 0;                        // phases of s_ready and o_done; blocks of the works before this
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&ms.work_full[it & 1], (it >> 1) & 1, wt, kSiteWork, it));
+      if (!ok) break;
+      const Work k = ms.work[it & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ms.work_empty[it & 1]);
+      if (!k.live) break;
+      const int lim = p.causal ? min(k.nk, k.lim0 + rr) : k.nk;
+      const int low = p.causal ? min(k.nk, k.lim0 + kRows * t) : k.nk;       // what the tile's first row sees
+      float m = kMInit, l = 0.f;
+      for (int i = 0; i < k.n[t]; ++i, ++ns) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[t], ns & 1, wt, kSiteS, i));
+        if (!ok) break;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld32(s_col + 32 * x, s + 32 * x);
+        tmem_wait_ld();
+        const int key0 = (k.b0 + i) * kBlock;
+        if (key0 + kBlock > low) {
+          const int seen = lim - key0;
+#pragma unroll
+          for (int x = 0; x < 128; ++x) s[x] = x < seen ? s[x] : -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mx[x] = fmaxf(s[x], s[x + 4]);
+#pragma unroll
+        for (int x = 8; x < 128; x += 8)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], fmaxf(s[x + y], s[x + y + 4]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (i == 0) {
+          m = fmaxf(m, top);
+        } else if (__any_sync(0xffffffffu, (top - m) * c > kOvershoot)) {      // (the S that is here is behind the PV before it)
+          const float now = fmaxf(m, top), f = fast_exp2((m - now) * c);
+          m = now;
+          l *= f;
+#pragma unroll 1
+          for (int x = 0; x < 128; x += 32) {
+            float o[32];
+            tmem_ld32(o_col + x, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tmem_st32(o_col + x, o);
+          }
+        }
+        const float mc = -m * c;
+        const uint64_t m2 = pack2(mc, mc);
+        uint64_t sum[2] = {0, 0};
+#pragma unroll
+        for (int x = 0; x < 128; x += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const float2 e = unpack2(fma2(pack2(s[x + 2 * y], s[x + 2 * y + 1]), c2, m2));
+            const float a = fast_exp2(e.x), b = fast_exp2(e.y);
+            sum[y & 1] = add2(sum[y & 1], pack2(a, b));
+            w[y] = bf16x2(a, b);
+          }
+          tmem_st16(s_col + x / 2, w);
+        }
+        const float2 both = unpack2(add2(sum[0], sum[1]));
+        l += both.x + both.y;
+        tmem_wait_st();
+        const int valid = k.nk - key0;
+        if (valid < kBlock) {
+          // Value rows behind the sequence's end: zeros, whatever lies there.  (Both tiles write them; the block's other granules are
+          // in nobody's way, and the slots are not given back before this tile's PV.)
+          const int from = max(valid, 0);
+#pragma unroll 1
+          for (int j = 3; j < kPerBlock; ++j) {
+            const int g = kPerBlock * (block0 + i) + j;
+            ok = __all_sync(0xffffffffu, mbar_wait(&ms.full[g & 7], (g >> 3) & 1, wt, kSiteFull, i)) && ok;
+            const uint32_t base = sbase + kOffRing + (uint32_t)(g & 7) * kGranule;
+            for (int x = r; x < (kBlock - from) * 8; x += kRows)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + from * 128 + 16 * x), "r"(0) : "memory");
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.p_ready[t]);
+      }
+      if (!ok) break;
+      block0 += max(k.n[0], k.n[1]);
+      // epilogue
+      const bool mine = rr < k.rows;
+      const long long row = (long long)(k.q0 + rr) * p.heads + k.head, prow = (long long)k.part * kPair + rr;
+      if (k.n[t] > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&ms.o_done[t], no & 1, wt, kSiteO, it));
+        if (!ok) break;
+        ++no;
+        tc_fence_after();
+      }
+      const float f = l > 0.f ? 1.f / l : 0.f;
+      if (mine) {
+        if (k.part < 0) p.lse[row] = l > 0.f ? (m * c + __log2f(l)) * kLn2 : INFINITY;
+        else p.part_ml[prow] = make_float2(m * c, l);
+      }
+      if (k.part < 0) {
+        uint4* dst = reinterpret_cast<uint4*>(p.out + row * (2 * kDV));
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          float o[32];
+          if (k.n[t] > 0) {                                                 // warp-uniform
+            tmem_ld32(o_col + 32 * x, o);
+            tmem_wait_ld();
+          }
+          if (mine) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              uint32_t w[4];
+#pragma unroll
+              for (int z = 0; z < 4; ++z) w[z] = l > 0.f ? bf16x2(o[8 * y + 2 * z] * f, o[8 * y + 2 * z + 1] * f) : 0u;   // without keys: 0
+              dst[4 * x + y] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      } else if (k.n[t] > 0) {
+        float4* dst = reinterpret_cast<float4*>(p.part_o + prow * kDV);
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          float o[32];
+          tmem_ld32(o_col + 32 * x, o);
+          tmem_wait_ld();
+          if (mine)
+#pragma unroll
+            for (int y = 0; y < 8; ++y) dst[8 * x + y] = make_float4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+  } else {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+   if (warp == kWarpMma) {
+    // ------------------------------------------------------------ the products (one thread)
+    if (lane == 0) {
+      constexpr uint32_t idesc_qk = umma_idesc(1, 1, false, false, 128, 128), idesc_pv = umma_idesc(1, 1, false, true, 128, 128),
+                         idesc_half = umma_idesc(1, 1, false, true, 128, 64);
+      const uint64_t q_desc = umma_desc(sbase + kOffQ, 16, 1024, kSwz128), k_desc = umma_desc(sbase + kOffRing, 16, 1024, kSwz128),
+                     v_desc = umma_desc(sbase + kOffRing, kGranule, 1024, kSwz128);
+      int block0 = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+      bool ok = true;
+      for (int it = 0; ok; ++it) {
+        if (!(ok = mbar_wait(&ms.work_full[it & 1], (it >> 1) & 1, wt, kSiteWork, it))) break;
+        const Work& k = ms.work[it & 1];
+        const int n0 = k.n[0], n1 = k.n[1], live = k.live, n = max(n0, n1);
+        mbar_arrive(&ms.work_empty[it & 1]);
+        if (!live) break;
+        auto count = [&](int t) { return t ? n1 : n0; };
+        auto last_user = [&](int t, int i) { return t == (i < n1 ? 1 : 0); };
+        auto qk = [&](int t, int i) {
+          for (int j = 0; j < 3; ++j) {
+            const int g = kPerBlock * (block0 + i) + j;
+            if (!(ok = mbar_wait(&ms.full[g & 7], (g >> 3) & 1, wt, kSiteFull, i))) return;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              mma_ss(tmem + 128 * t, q_desc + ((kQTile * t + kGranule * j) >> 4) + 2 * x, k_desc + (uint32_t)(g & 7) * (kGranule >> 4) + 2 * x, idesc_qk,
+                     (uint32_t)(j | x));
+            if (last_user(t, i)) mma_commit_cta(&ms.empty[g & 7]);
+          }
+          mma_commit_cta(&ms.s_ready[t]);
+          if (i + 1 == count(t)) mma_commit_cta(&ms.q_free[t]);
+        };
+        auto pv = [&](int t, int i) {
+          if (!(ok = mbar_wait(&ms.p_ready[t], np[t] & 1, wt, kSiteP, i))) return;
+          ++np[t];
+          const int g = kPerBlock * (block0 + i) + 3;
+          for (int j = 0; j < 2; ++j)
+            if (!(ok = mbar_wait(&ms.full[(g + j) & 7], ((g + j) >> 3) & 1, wt, kSiteFull, i))) return;
+          tc_fence_after();
+          const uint32_t d = tmem + kTmemO + 128 * t, a = tmem + 128 * t;
+          const uint64_t v0 = v_desc + (uint32_t)(g & 7) * (kGranule >> 4);
+          if ((g & 7) != 7) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) mma_ts(d, a + 8 * x, v0 + 128 * x, idesc_pv, (uint32_t)(i | x));
+          } else {                                            // the block's two granules of V lie at the ring's two ends
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int x = 0; x < 8; ++x) mma_ts(d + 64 * j, a + 8 * x, (j ? v_desc : v0) + 128 * x, idesc_half, (uint32_t)(i | x));
+          }
+          if (last_user(t, i))
+            for (int j = 0; j < 2; ++j) mma_commit_cta(&ms.empty[(g + j) & 7]);
+          if (i + 1 == count(t)) mma_commit_cta(&ms.o_done[t]);
+        };
+        for (int t = 0; t < 2 && ok; ++t)
+          if (count(t) > 0) {
+            if ((ok = mbar_wait(&ms.q_full[t], nq[t] & 1, wt, kSiteQ, it))) { ++nq[t]; qk(t, 0); }
+          }
+        // Q_t K(i + 1) writes S over the P that P_t V(i) reads.  Both are issued by this thread, and a CTA's products go through its
+        // tensor core in the order of issue: the reads of the earlier are behind it when the later's first results are written.
+        for (int i = 0; i < n && ok; ++i)
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (i < count(t)) pv(t, i);
+            if (ok && i + 1 < count(t)) qk(t, i + 1);
+          }
+        block0 += n;
+      }
+      if (!ok) {                                              // given up: what has been issued ends before the tensor memory goes
+        mma_commit_cta(&ms.drained);
+        mbar_drain(&ms.drained, 0);
+      }
+    }
+    __syncwarp();
+   } else if (warp == kWarpLoad) {
+    // ------------------------------------------------------------ work and loads (one warp; lane 0 waits and issues)
+    const int tiles_all = tiles * p.heads;
+    const Cut cut = cut_of(tiles_all, most, p, lane);
+    const uint64_t once = l2_policy_evict_first();
+    uint64_t keep;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(keep));
+    int w = (int)blockIdx.x, block0 = 0, asked = 0, nq[2] = {0, 0}, clc_asked = 0, clc_got = 0;
+    bool ok = true;
+    for (int it = 0; ok;) {
+      if (w == 0 && lane == 0 && p.plan) *p.plan = make_int4(tiles, cut.whole, cut.pieces, 0);
+      Work k;
+      k.live = 0;
+      if (w >= 0) k = work_of(w, tiles, cut, p, lane);
+      if (w >= 0 && lane == 0) {                              // ask for the next while this one is loaded
+        fence_proxy_async_smem();
+        mbar_arrive_expect_tx(&ms.clc, 16);
+        clc_ask(&ms.clc_answer, &ms.clc);
+      }
+      if (w >= 0) ++clc_asked;
+      if (k.live || w < 0) {
+        if (lane == 0) {
+          ok = it < 2 || mbar_wait(&ms.work_empty[it & 1], ((it >> 1) & 1) ^ 1, wt, kSiteWorkEmpty, it);
+          if (ok) {
+            ms.work[it & 1] = k;
+            mbar_arrive(&ms.work_full[it & 1]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (!ok || w < 0) break;
+        if (lane == 0) {
+          for (int t = 0; t < 2 && ok; ++t)
+            if (k.n[t] > 0) {
+              if (nq[t] > 0 && !(ok = mbar_wait(&ms.q_free[t], (nq[t] - 1) & 1, wt, kSiteQFree, it))) break;
+              mbar_arrive_expect_tx(&ms.q_full[t], kQTile);
+              for (int j = 0; j < 3; ++j)
+                tma_load_3d_hint(sbase + kOffQ + kQTile * t + kGranule * j, &map_q, 64 * j, k.head, k.q0 + kRows * t, &ms.q_full[t], once);
+              ++nq[t];
+            }
+          const int n = max(k.n[0], k.n[1]);
+          for (int i = 0; i < n && ok; ++i) {
+            const int at = k.k0 + (k.b0 + i) * kBlock;
+            for (int j = 0; j < kPerBlock; ++j) {
+              const int g = kPerBlock * (block0 + i) + j;
+              uint64_t* bar = &ms.full[g & 7];
+              const uint32_t dst = sbase + kOffRing + (uint32_t)(g & 7) * kGranule;
+              if (g >= kRing && !(ok = mbar_wait(&ms.empty[g & 7], ((g >> 3) & 1) ^ 1, wt, kSiteEmpty, i))) break;
+              mbar_arrive_expect_tx(bar, kGranule);
+              if (j < 2) tma_load_3d_hint(dst, &map_kn, 64 * j, k.head, at, bar, keep);
+              else if (j == 2) tma_load_2d_hint(dst, &map_kr, 0, at, bar, keep);
+              else tma_load_3d_hint(dst, &map_v, 64 * (j - 3), k.head, at, bar, keep);
+              asked = g + 1;
+            }
+          }
+          block0 += n;
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        ++it;
+      }
+      if (!ok) break;
+      int next = -1;
+      if (lane == 0) {
+        ok = mbar_wait(&ms.clc, clc_got & 1, wt, kSiteClc, it);
+        if (ok) next = clc_block(&ms.clc_answer);
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (ok) ++clc_got;
+      w = __shfl_sync(0xffffffffu, next, 0);
+    }
+    if (!ok && lane == 0) {                                   // given up: what is in flight lands first
+      for (int g = max(asked - kRing, 0); g < asked; ++g) mbar_drain(&ms.full[g & 7], (g >> 3) & 1);
+      for (int t = 0; t < 2; ++t)
+        if (nq[t] > 0) mbar_drain(&ms.q_full[t], (nq[t] - 1) & 1);
+      if (clc_asked > clc_got) mbar_drain(&ms.clc, clc_got & 1);
+    }
+    __syncwarp();
+   }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma) tmem_dealloc_cta(tmem, 512);
+  if (threadIdx.x == 0) {
+    wt.report(g_status, p.epoch);
+    if (blockIdx.x == 0) atomicAdd(&g_status[3], 1);
+  }
+}
+
+// out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the pieces of cut tile blockIdx.y; a warp has a row, eight pieces' loads under way
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(32 * kMergeWarps) mla_prefill_merge_kernel(const Params p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
+  const int4 plan = __ldcg(p.plan);
+  const Cut cut{plan.y, plan.z};
+  const int w0 = cut.whole + (int)blockIdx.y * cut.pieces, rr = (int)blockIdx.x * kMergeWarps + warp;
+  if (cut.pieces < 2 || cut.whole + (int)blockIdx.y >= plan.x * p.heads) return;
+  const Work k = work_of(w0, plan.x, cut, p, lane);
+  if (!k.live || rr >= k.rows) return;
+  const long long base = (long long)k.part * kPair + rr;
+  float m = kMInit;
+  for (int i = lane; i < cut.pieces; i += 32) {
+    const float2 ml = __ldcg(p.part_ml + base + (long long)i * kPair);
+    if (ml.y > 0.f) m = fmaxf(m, ml.x);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i0 = 0; i0 < cut.pieces; i0 += 8) {
+    float4 v[8];
+    float2 ml[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      ml[u] = make_float2(0.f, 0.f);
+      if (i0 + u < cut.pieces) {
+        const long long at = base + (long long)(i0 + u) * kPair;
+        ml[u] = __ldcg(p.part_ml + at);
+        v[u] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * kDV) + lane);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (!(ml[u].y > 0.f)) continue;                         // beyond the list, or a piece without keys for this row
+      const float f = fast_exp2(ml[u].x - m);
+      l += f * ml[u].y;
+      a.x += f * v[u].x; a.y += f * v[u].y; a.z += f * v[u].z; a.w += f * v[u].w;
+    }
+  }
+  const float f = l > 0.f ? 1.f / l : 0.f;
+  const long long row = (long long)(k.q0 + rr) * p.heads + k.head;
+  reinterpret_cast<uint2*>(p.out + row * (2 * kDV))[lane] = make_uint2(bf16x2(a.x * f, a.y * f), bf16x2(a.z * f, a.w * f));
+  if (lane == 0) p.lse[row] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+}
+
+// Pieces that a call's workspace holds: none where its tiles are known to be many, or its sequences too short to be cut.
+static int pieces_of(int Tq, int Tk, int heads) {
+  const int ctas = sm_count();
+  const int64_t tiles = (int64_t)((Tq + kPair - 1) / kPair) * heads;
+  return tiles > 4 * ctas || blocks_seen(Tk) < 4 ? 0 : 4 * ctas;
+}
+
+}  // namespace prefill
+}  // namespace lt
+
+extern "C" int64_t litedsa_mla_prefill_workspace(int Tq, int Tk, int heads) {
+  if (Tq <= 0 || Tk <= 0 || heads <= 0) return 0;
+  const int64_t n = lt::prefill::pieces_of(Tq, Tk, heads);
+  return n == 0 ? 0 : 16 + n * lt::prefill::kPair * (lt::prefill::kDV * 4 + 8);
+}
+
+extern "C" int litedsa_mla_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_nope, int64_t k_token_stride,
+                                   int64_t k_head_stride, const void* k_rope, int64_t k_rope_stride, const void* v, int64_t v_token_stride,
+                                   int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int B, float sm_scale, int causal, void* out,
+                                   float* lse, int Tq, int Tk, int heads, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace lt;
+  using namespace lt::prefill;
+  if (!q || !out || !lse || (Tk > 0 && (!k_nope || !k_rope || !v)) || (cu_q == nullptr) != (cu_k == nullptr)) {
+    if (Tq != 0) return LITEDSA_ERR_ARG;
+  }
+  if (Tq < 0 || Tk < 0 || heads <= 0 || B < 0 || (!cu_q && B != 1)) return LITEDSA_ERR_SHAPE;
+  if (!(sm_scale >= 0.f)) return LITEDSA_ERR_UNSUPPORTED;
+  if (((uintptr_t)q | (uintptr_t)k_nope | (uintptr_t)k_rope | (uintptr_t)v | (uintptr_t)out | (uintptr_t)workspace) & 15 || ((uintptr_t)lse & 3) ||
+      (q_token_stride | q_head_stride | k_token_stride | k_head_stride | k_rope_stride | v_token_stride | v_head_stride) % 8)
+    return LITEDSA_ERR_UNSUPPORTED;
+  if (Tq == 0 || B == 0) return LITEDSA_OK;
+  const int64_t tiles = cu_q ? min((int64_t)Tq, Tq / kPair + (int64_t)B) : (Tq + kPair - 1) / kPair;
+  Params p = {};
+  p.max_pieces = pieces_of(Tq, Tk, heads);
+  if (tiles * heads + p.max_pieces >= (1ll << 31) - 1) return LITEDSA_ERR_UNSUPPORTED;
+  const int64_t need = litedsa_mla_prefill_workspace(Tq, Tk, heads);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return workspace ? LITEDSA_ERR_SHAPE : LITEDSA_ERR_ARG;
+  p.cu_q = cu_q; p.cu_k = cu_k;
+  p.out = reinterpret_cast<uint8_t*>(out); p.lse = lse;
+  if (p.max_pieces) {
+    p.plan = reinterpret_cast<int4*>(workspace);
+    p.part_o = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 16);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)p.max_pieces * kPair * kDV);
+  }
+  p.B = B; p.Tq = Tq; p.Tk = Tk; p.heads = heads; p.ctas = sm_count(); p.causal = causal != 0;
+  p.scale_log2 = fmaxf(sm_scale * kLog2e, 1e-30f);           // not 0: masked scores are -inf before they are scaled
+  p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const auto bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap mq, mn, mr, mv;
+  // strides of dimensions of one are never used, but have to be such as a map can hold
+  auto pitch = [](int64_t elements, int64_t n, int64_t least) -> uint64_t { return (uint64_t)(2 * (n > 1 ? elements : least)); };
+  if (!make_map_3d(&mq, q, bf16, 192, heads, Tq, pitch(q_head_stride, heads, 192), pitch(q_token_stride, Tq, 192), 64, 1, kRows)) return LITEDSA_ERR_CUDA;
+  mn = mr = mv = mq;
+  if (Tk > 0 && (!make_map_3d(&mn, k_nope, bf16, 128, heads, Tk, pitch(k_head_stride, heads, 128), pitch(k_token_stride, Tk, 128), 64, 1, kBlock) ||
+                 !make_map_2d(&mr, k_rope, bf16, 64, Tk, pitch(k_rope_stride, Tk, 64), 64, kBlock) ||
+                 !make_map_3d(&mv, v, bf16, 128, heads, Tk, pitch(v_head_stride, heads, 128), pitch(v_token_stride, Tk, 128), 64, 1, kBlock)))
+    return LITEDSA_ERR_CUDA;
+  if (!ensure_smem<mla_prefill_kernel>(current_device(), kSmem)) return LITEDSA_ERR_CUDA;
+  const int rc = launch_pdl(mla_prefill_kernel, dim3((unsigned)(tiles * heads + p.max_pieces)), kThreads, kSmem, st, mq, mn, mr, mv, p);
+  if (rc != LITEDSA_OK || p.max_pieces == 0) return rc;
+  return launch_pdl(mla_prefill_merge_kernel, dim3(kPair / kMergeWarps, (unsigned)min(tiles * heads, (int64_t)p.ctas)), 32 * kMergeWarps, 0, st, p);
+}
+
+// Status block of the kernel; layout and return rule as litedsa_attn_status.
+extern "C" int litedsa_mla_prefill_status(int* out4_host, int reset) {
+  using namespace lt::prefill;
+  if (out4_host && cudaMemcpyFromSymbol(out4_host, g_status, sizeof(int) * 4) != cudaSuccess) return LITEDSA_ERR_CUDA;
+  if (reset) {
+    const int z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (cudaMemcpyToSymbol(g_status, z, sizeof(z)) != cudaSuccess) return LITEDSA_ERR_CUDA;
+  }
+  return (out4_host && out4_host[0] != 0) ? LITEDSA_ERR_TIMEOUT : LITEDSA_OK;
+}

@@ -1,7 +1,7 @@
-"""The dense side of latent attention: writing the paged cache and attending to all of it.
+"""The dense side of latent attention: writing the paged cache, attending to all of it, and the prefill of prompts.
 
 ``append_kv`` writes the rows that ``mla_decode`` reads (and, flattened to ``[rows, 656]`` or ``[rows, 576]``, that
-``prepare_kv`` and ``sparse_prefill`` take).
+``prepare_kv`` and ``sparse_prefill`` take); ``mla_prefill`` is the expanded form, over keys and values of every head.
 
 Like the operators of :mod:`litetopk_b200.api` these are thin wrappers over the C ABI: asynchronous on the current stream of
 their tensors' device, checked here and in C, without a CPU path, and without host synchronisation, so that they can be captured in a
@@ -150,3 +150,62 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tenso
 def mla_decode_status(reset: bool = False, device=None):
     """Status block of the decode kernel (see :func:`litetopk_b200.attn_status`)."""
     return _status("litedsa_mla_decode_status", reset, device)
+
+
+def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: torch.Tensor, sm_scale: float, *,
+                cu_seqlens_q: Optional[torch.Tensor] = None, cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True,
+                out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+    """Expanded latent attention over a batch of sequences: scores ``sm_scale * (q[..., :128] . k_nope + q[..., 128:] . k_rope)``.
+
+    q [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64] (one for all heads), all bf16; any strides that are multiples
+    of 8 with unit inner stride (k_nope and v may be views of one projection).  Sequence b has queries ``cu_seqlens_q[b] : cu_seqlens_q[b + 1]`` and
+    keys ``cu_seqlens_k[b] : cu_seqlens_k[b + 1]`` (int32 [B + 1]; both None: one sequence of all).  ``causal``: its queries are its last tokens,
+    query i of n sees the first ``m - n + 1 + i`` of its m keys.  ``sm_scale`` must not be negative.
+
+    Returns ``(out [Tq, heads, 128] bf16, lse [Tq, heads] f32)``, written into ``out`` / ``lse`` when given (contiguous).  A row that sees
+    no key: out = 0, lse = +inf.  Rows that are no sequence's (behind ``cu_seqlens_q[-1]``) are not written.
+    """
+    for t, n, d in ((q, "q", 3), (k_nope, "k_nope", 3), (k_rope, "k_rope", 2), (v, "v", 3)):
+        _need(t, n, torch.bfloat16, d)
+        if t.stride(-1) != 1:
+            raise ValueError(f"{n} needs unit inner stride")
+    dev, (Tq, heads, d), Tk = q.device, q.shape, k_rope.shape[0]
+    if d != 192 or heads < 1 or k_nope.shape != (Tk, heads, 128) or v.shape != (Tk, heads, 128) or k_rope.shape[1] != 64:
+        raise ValueError("q must be [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64]")
+    if not sm_scale >= 0:
+        raise ValueError("sm_scale must not be negative")
+    B = 1
+    if (cu_seqlens_q is None) != (cu_seqlens_k is None):
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must be given together")
+    if cu_seqlens_q is not None:
+        _need(cu_seqlens_q, "cu_seqlens_q", torch.int32, 1)
+        _need(cu_seqlens_k, "cu_seqlens_k", torch.int32, 1)
+        B = cu_seqlens_q.shape[0] - 1
+        if B < 0 or cu_seqlens_k.shape[0] != B + 1 or not (cu_seqlens_q.is_contiguous() and cu_seqlens_k.is_contiguous()):
+            raise ValueError("cu_seqlens_q and cu_seqlens_k must be contiguous [B + 1]")
+    if out is None:
+        out = _empty((Tq, heads, 128), torch.bfloat16, dev)
+    else:
+        _need(out, "out", torch.bfloat16)
+        if out.shape != (Tq, heads, 128) or not out.is_contiguous():
+            raise ValueError("out must be a contiguous [Tq, heads, 128] bf16 tensor")
+    if lse is None:
+        lse = _empty((Tq, heads), torch.float32, dev)
+    else:
+        _need(lse, "lse", torch.float32)
+        if lse.shape != (Tq, heads) or not lse.is_contiguous():
+            raise ValueError("lse must be a contiguous [Tq, heads] f32 tensor")
+    _same_device(dev, k_nope=k_nope, k_rope=k_rope, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k, out=out, lse=lse)
+    if Tq == 0 or B == 0:
+        return out, lse
+    need = _workspace_bytes("litedsa_mla_prefill_workspace", dev.index, Tq, Tk, heads)
+    ws = _empty((need,), torch.uint8, dev) if need else None
+    check(_on_device(dev, _lib.lib().litedsa_mla_prefill, _ptr(q), q.stride(0), q.stride(1), _ptr(k_nope), k_nope.stride(0), k_nope.stride(1),
+                     _ptr(k_rope), k_rope.stride(0), _ptr(v), v.stride(0), v.stride(1), _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), B,
+                     float(sm_scale), bool(causal), _ptr(out), _ptr(lse), Tq, Tk, heads, _ptr(ws), need), "mla_prefill")
+    return out, lse
+
+
+def mla_prefill_status(reset: bool = False, device=None):
+    """Status block of the prefill kernel (see :func:`litetopk_b200.attn_status`)."""
+    return _status("litedsa_mla_prefill_status", reset, device)

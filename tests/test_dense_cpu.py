@@ -40,6 +40,22 @@ def test_decode_refuses_wrong_arguments(built_lib):
     assert built_lib.litedsa_mla_decode_workspace(0, 16) == built_lib.litedsa_mla_decode_workspace(1, 129) == 0
 
 
+def test_prefill_refuses_wrong_arguments(built_lib):
+    def call(q=P, kn=P, kr=P, v=P, cq=P, ck=P, B=2, scale=0.1, out=P, lse=P, Tq=1 << 20, Tk=100, heads=16, ws=None, size=0, qs=3200):
+        return built_lib.litedsa_mla_prefill(q, qs, 192, kn, 4096, 256, kr, 64, v, 4096, 256, cq, ck, B, scale, 1, out, lse, Tq, Tk, heads, ws, size, None)
+    for name in ("q", "kn", "kr", "v", "cq", "ck", "out", "lse"):
+        assert call(**{name: None}) == _lib.ERR_ARG, name
+    for bad in (dict(B=-1), dict(cq=None, ck=None), dict(Tq=-1), dict(Tk=-1), dict(heads=0)):
+        assert call(**bad) == _lib.ERR_SHAPE, bad
+    for bad in (dict(scale=-0.1), dict(scale=math.nan), dict(q=P + 8), dict(kn=P + 8), dict(kr=P + 8), dict(v=P + 8), dict(out=P + 8), dict(lse=P + 2),
+                dict(qs=3204), dict(Tq=(1 << 31) - 1, heads=1 << 10)):
+        assert call(**bad) == _lib.ERR_UNSUPPORTED, bad
+    assert call(Tq=0) == call(Tq=0, q=None, out=None, lse=None) == _lib.OK
+    need = built_lib.litedsa_mla_prefill_workspace(64, 4096, 2)
+    assert need > 0 and built_lib.litedsa_mla_prefill_workspace(8192, 8192, 64) == built_lib.litedsa_mla_prefill_workspace(64, 64, 2) == 0
+    assert call(Tq=64, Tk=4096, heads=2) == _lib.ERR_ARG and call(Tq=64, Tk=4096, heads=2, ws=P, size=need - 1) == _lib.ERR_SHAPE
+
+
 def test_python_layer_names_what_is_wrong():
     import litetopk_b200 as lt
     cpu = torch.zeros((2, 512), dtype=torch.bfloat16)

@@ -327,3 +327,167 @@ def test_append_to_nothing():
     assert torch.equal(k_out, kr)                                     # a cache without rows: the token is padding
     lt.append_kv(kv, kr, z, torch.zeros((0, 64), device=DEV), z, torch.zeros((4, 656), dtype=torch.uint8, device=DEV), k_out=k_out.zero_())
     assert bool((k_out == 0).all())                                   # no positions: it is left out
+
+
+# --------------------------------------------------------------------------- mla_prefill
+def _ragged(g, lq, lk, heads, gap=0, scale=1.0):
+    """Operands of sequences of these lengths, ``gap`` rows of NaN and infinities behind each sequence's keys."""
+    cu_q = [0]
+    for n in lq:
+        cu_q.append(cu_q[-1] + n)
+    Tk = sum(lk) + gap * len(lk)
+    kv = _bf16(g, Tk, heads, 256, scale=scale)
+    rope = _bf16(g, Tk, 64)
+    q = _bf16(g, cu_q[-1], heads, 192)
+    starts, at = [], 0
+    for n in lk:
+        starts.append(at)
+        kv[at + n:at + n + gap] = torch.tensor([math.nan, math.inf, -math.inf])[torch.arange(gap * heads * 256) % 3].view(gap, heads, 256).to(torch.bfloat16)
+        rope[at + n:at + n + gap] = math.nan
+        at += n + gap
+    return q, kv, rope, cu_q, starts
+
+
+def _prefill_compare(q, kv, rope, cu_q, starts, lk, got, causal=True, heads=None, rows=None, scale=SCALE):
+    out, lse = got
+    assert lt.mla_prefill_status(reset=True)[0] == 0
+    heads = list(range(q.shape[1])) if heads is None else heads
+    out, lse = out.cpu()[:, heads], lse.cpu()[:, heads]
+    for b in range(len(lk)):
+        n, m, k0 = cu_q[b + 1] - cu_q[b], lk[b], starts[b]
+        k, v, r = kv[k0:k0 + m][:, heads, :128], kv[k0:k0 + m][:, heads, 128:], rope[k0:k0 + m]
+        pick = range(n) if rows is None else sorted({x for x in rows if x < n} | ({n - 1} if n else set()))
+        for i in pick:
+            see = max(0, m - n + 1 + i) if causal else m
+            o, s, o_tol, s_tol = do.prefill(q[cu_q[b] + i:cu_q[b] + i + 1][:, heads], k[:see], r[:see], v[:see], scale, causal=False)
+            _check(out[cu_q[b] + i:cu_q[b] + i + 1], o, o_tol)
+            _check(lse[cu_q[b] + i:cu_q[b] + i + 1], s, s_tol)
+
+
+def _cu(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,m,heads", [(1, 1, 1), (1, 300, 3), (77, 77, 2), (128, 128, 1), (129, 129, 2), (130, 257, 1), (257, 257, 1), (300, 700, 2),
+                                       (5, 3, 2), (200, 60, 1), (3, 0, 2)])
+def test_prefill_of_one_sequence(causal, n, m, heads):
+    g = _gen(n + m)
+    q, kv, rope, cu_q, starts = _ragged(g, [n], [m], heads)
+    kd = kv.to(DEV)
+    got = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE, causal=causal)
+    _prefill_compare(q, kv, rope, cu_q, starts, [m], got, causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_of_a_ragged_batch_beside_numbers_that_are_none(causal):
+    g = _gen(17)
+    lq, lk, heads = [3, 0, 130, 1, 260, 40, 7], [3, 5, 130, 400, 300, 11, 0], 3
+    q, kv, rope, cu_q, starts = _ragged(g, lq, lk, heads, gap=2)
+    kd = kv.to(DEV)
+    # a sequence's keys end where the gap begins: its cu_seqlens_k entry and the next one's differ, so the gaps are sequences without queries
+    cq, ck = [0], [0]
+    for b in range(len(lq)):
+        cq += [cu_q[b + 1], cu_q[b + 1]]
+        ck += [starts[b] + lk[b], starts[b] + lk[b] + 2]
+    got = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE, cu_seqlens_q=_cu(cq), cu_seqlens_k=_cu(ck), causal=causal)
+    _prefill_compare(q, kv, rope, cu_q, starts, lk, got, causal)
+
+
+@pytest.mark.parametrize("n,m,heads", [(6, 4718, 1), (300, 9001, 2), (1500, 4096, 5)])
+def test_prefill_cuts_few_tiles_along_the_keys(n, m, heads):
+    g = _gen(n)
+    q, kv, rope, cu_q, starts = _ragged(g, [n], [m], heads)
+    kd = kv.to(DEV)
+    got = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE)
+    _prefill_compare(q, kv, rope, cu_q, starts, [m], got, heads=sorted({0, heads - 1}), rows={0, 127, 128, 255, 256, 700, 1279})
+
+
+def test_prefill_deals_out_many_tiles():
+    g = _gen(23)
+    lq = [900, 1, 513] + [17] * 60
+    lk = [1000, 130, 513] + [40] * 60
+    heads = 40                                                       # 63 sequences: 67 tiles a head
+    q, kv, rope, cu_q, starts = _ragged(g, lq, lk, heads)
+    kd = kv.to(DEV)
+    cu_k = [0]
+    for m in lk:
+        cu_k.append(cu_k[-1] + m)
+    args = (q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE)
+    got = lt.mla_prefill(*args, cu_seqlens_q=_cu(cu_q), cu_seqlens_k=_cu(cu_k))
+    _prefill_compare(q, kv, rope, cu_q, starts, lk, got, heads=[0, 21, 39], rows={0, 130, 256, 600})
+    again = lt.mla_prefill(*args, cu_seqlens_q=_cu(cu_q), cu_seqlens_k=_cu(cu_k))
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("rising", [1.0, -1.0, 0.0])
+def test_prefill_follows_a_moving_maximum(rising):
+    g = _gen(29)
+    n, m, heads = 200, 1300, 2
+    q, kv, rope, cu_q, starts = _ragged(g, [n], [m], heads)
+    ramp = rising * torch.arange(m) / 3.0 if rising else torch.where(torch.arange(m) % 97 == 3, 300.0, -300.0)
+    rope[:, 0] = ramp.to(torch.bfloat16)
+    q[:, :, 128] = torch.linspace(-5, 14, n).to(torch.bfloat16)[:, None]
+    kd = kv.to(DEV)
+    got = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE)
+    _prefill_compare(q, kv, rope, cu_q, starts, [m], got, rows=set(range(0, 200, 9)))
+    got = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], 0.0)
+    _prefill_compare(q, kv, rope, cu_q, starts, [m], got, rows={0, 150}, scale=0.0)
+
+
+def test_prefill_takes_views_given_outputs_and_leaves_other_rows():
+    g = _gen(31)
+    lq, lk, heads = [20, 33], [50, 33], 5
+    q, kv, rope, cu_q, starts = _ragged(g, lq, lk, heads)
+    Tq, Tk = 53 + 9, 83 + 4
+    q_wide = torch.full((Tq, 8, 200), math.nan, dtype=torch.bfloat16)
+    q_wide[:53, :heads, :192] = q
+    kn = torch.full((Tk, 8, 136), math.nan, dtype=torch.bfloat16)
+    vv, rr = kn.clone(), torch.full((Tk, 72), math.nan, dtype=torch.bfloat16)
+    kn[:83, :heads, :128], vv[:83, :heads, :128], rr[:83, :64] = kv[..., :128], kv[..., 128:], rope
+    out = torch.full((Tq, heads, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    lse = torch.full((Tq, heads), 5.0, device=DEV)
+    got = lt.mla_prefill(q_wide.to(DEV)[:, :heads, :192], kn.to(DEV)[:, :heads, :128], rr.to(DEV)[:, :64], vv.to(DEV)[:, :heads, :128], SCALE,
+                         cu_seqlens_q=_cu([0, 20, 53]), cu_seqlens_k=_cu([0, 50, 83]), out=out, lse=lse)
+    assert got[0].data_ptr() == out.data_ptr()
+    _prefill_compare(q, kv, rope, cu_q, starts, lk, (out[:53], lse[:53]))
+    assert bool((out[53:] == 5).all()) and bool((lse[53:] == 5).all())
+
+
+def test_prefill_in_graphs_follows_new_lengths():
+    g = _gen(37)
+    heads, T = 2, 700
+    q, kv, rope, _, _ = _ragged(g, [T], [T], heads)
+    qd, kd, rd = q.to(DEV), kv.to(DEV), rope.to(DEV)
+    cq, ck = _cu([0, 300, T]), _cu([0, 300, T])
+    lt.mla_prefill(qd, kd[..., :128], rd, kd[..., 128:], SCALE, cu_seqlens_q=cq, cu_seqlens_k=ck)
+    side, graphs, got = torch.cuda.Stream(), [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    with torch.cuda.stream(side):
+        for x in graphs:
+            with torch.cuda.graph(x, stream=side):
+                got.append(lt.mla_prefill(qd, kd[..., :128], rd, kd[..., 128:], SCALE, cu_seqlens_q=cq, cu_seqlens_k=ck))
+    torch.cuda.synchronize()
+    for cuts in (([0, 300, 700], [0, 300, 700]), ([0, 0, 513], [0, 100, 700]), ([0, 1, 2], [0, 650, 700])):
+        cq.copy_(_cu(cuts[0]))
+        ck.copy_(_cu(cuts[1]))
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        end = cuts[0][-1]
+        assert torch.equal(got[0][0][:end], got[1][0][:end]) and torch.equal(got[0][1][:end], got[1][1][:end])
+        lk = [cuts[1][1], cuts[1][2] - cuts[1][1]]
+        _prefill_compare(q, kv, rope, cuts[0], cuts[1], lk, got[0], rows={0, 129, 255, 256, 299, 400})
+
+
+def test_prefill_of_nothing():
+    e = torch.zeros((0, 2, 192), dtype=torch.bfloat16, device=DEV)
+    kv, r = torch.zeros((4, 2, 256), dtype=torch.bfloat16, device=DEV), torch.zeros((4, 64), dtype=torch.bfloat16, device=DEV)
+    out, lse = lt.mla_prefill(e, kv[..., :128], r, kv[..., 128:], SCALE)
+    assert out.shape == (0, 2, 128) and lse.shape == (0, 2)
+    q = torch.ones((3, 2, 192), dtype=torch.bfloat16, device=DEV)
+    out = torch.full((3, 2, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    lt.mla_prefill(q, kv[..., :128], r, kv[..., 128:], SCALE, cu_seqlens_q=_cu([0]), cu_seqlens_k=_cu([0]), out=out)
+    lt.mla_prefill(q, kv[..., :128], r, kv[..., 128:], SCALE, cu_seqlens_q=_cu([0, 0, 0]), cu_seqlens_k=_cu([0, 2, 4]), out=out)
+    assert bool((out == 5).all())
