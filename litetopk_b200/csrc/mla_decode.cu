@@ -33,7 +33,8 @@ constexpr int kChunks = kD / 64;
 constexpr uint32_t kChunkBytes = kBlock * 128;              // 64 keys x 64 bf16
 constexpr uint32_t kSlotBytes = kChunks * kChunkBytes;
 constexpr int kSlots = 2;
-constexpr int kWarpMma = 4, kWarpLoad0 = 5, kPackedWarps = 8;
+constexpr int kGroups = 5;                                  // a tile's chunks are loaded and given back in groups: four of 128 dims, the rope dims
+constexpr int kWarpQk = 4, kWarpPv = 5, kWarpQ = 6, kWarpLoad0 = 7, kBf16Warps = 2, kPackedWarps = 8;
 constexpr int kPackedRow = 656;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMInit = -1e30f;
@@ -55,7 +56,7 @@ struct Plan {
 };
 
 struct Misc {
-  uint64_t kv_full[kSlots], s_ready[2], p_ready[2], pv_done[kSlots], q_ready, drained;
+  uint64_t kv_full[kSlots][kGroups], kv_free[kSlots][kGroups], s_ready[2], p_ready[2], q_ready, q_free, drained[2];
   uint32_t left, tmem_base;
   int start_b, start_k, count, meta_groups;
   long long start_pos, total;
@@ -77,6 +78,7 @@ struct Params {
   float* part_o;                  // [CTA][2][kRows][512]
   float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
   int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
+  int flat_q;                     // a sequence's rows are evenly spaced: they come by TMA
   int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows;
   float scale_log2;
   int epoch;
@@ -152,8 +154,8 @@ __device__ __forceinline__ void st_shared16(uint32_t a, const uint4& v) {
 __device__ __forceinline__ void st_shared4(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 
 template <int kRows, bool kPacked>
-__global__ void __launch_bounds__(kPacked ? 32 * (kWarpLoad0 + kPackedWarps) : 32 * (kWarpLoad0 + 1), 1)
-mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
+__global__ void __launch_bounds__(kPacked ? 32 * (kWarpLoad0 + kPackedWarps) : 32 * (kWarpLoad0 + kBf16Warps), 1)
+mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q, const Params p) {
   using PL = Plan<kRows>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 1023u) & ~1023u;      // swizzled tiles
@@ -164,16 +166,19 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
   const int g = (int)blockIdx.x / p.row_tiles, rt = (int)blockIdx.x - g * p.row_tiles;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) { mbar_init(&ms.kv_full[i], kPacked ? kPackedWarps : 1); mbar_init(&ms.pv_done[i], 1); }
+    for (int i = 0; i < kSlots; ++i)
+      for (int j = 0; j < kGroups; ++j) { mbar_init(&ms.kv_full[i][j], kPacked ? kPackedWarps : kBf16Warps); mbar_init(&ms.kv_free[i][j], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4); }
-    mbar_init(&ms.q_ready, 4);
-    mbar_init(&ms.drained, 1);
+    mbar_init(&ms.q_ready, 1);
+    mbar_init(&ms.q_free, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&ms.drained[i], 1);
     ms.left = 0;
     ms.count = 0;
     fence_mbar_init();
     if (!kPacked) tma_prefetch_desc(&map_kv);
+    if (p.flat_q) tma_prefetch_desc(&map_q);
   }
-  if (warp == kWarpMma) {
+  if (warp == kWarpQk) {
     tmem_alloc_cta(&ms.tmem_base, PL::kTmemCols);
     tmem_relinquish_cta();
   }
@@ -216,31 +221,15 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
   const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem_base, 0);
 
   if (warp < 4) {
-    // ------------------------------------------------------------ softmax, queries, epilogue
+    // ------------------------------------------------------------ softmax, epilogue
     // A warp has 16 rows: lane l rows l / 4 and l / 4 + 8, of every 8 keys the pair 2 (l % 4).
     const int r0 = 16 * warp + (lane >> 2), qd = lane & 3;
     const bool live = 16 * warp < kRows;
     const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
-    auto request_q = [&](int b) {
-      for (int i = (int)threadIdx.x; i < kRows * (kD / 8); i += 128) {
-        const int r = i / (kD / 8), c = i - r * (kD / 8), row = rt * kRows + r;
-        const uint32_t dst = sbase + PL::kOffQ + (uint32_t)(c >> 3) * PL::kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        const int j = row / p.heads, h = row - j * p.heads;
-        const bool in = row < p.rows;
-        cp_async16_or_zero(dst, p.q + (in ? b * p.q_b + j * p.q_j + h * p.q_h + 16 * c : 0), in);
-      }
-    };
-    auto pass_q = [&]() {
-      cp_async_wait_all();
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ms.q_ready);
-    };
     Walk w(ms);
     int kb = 0;
     // A wait here that gives up is passed like any other: the four warps meet at named barriers, so they take the same steps.
     bool more = w.next(p);
-    if (more) { request_q(w.b); pass_q(); }
     while (more) {
       // rows' limits
       int lim[2], low;
@@ -256,7 +245,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
       for (int k = w.k0; k < w.k1; ++k, ++kb) {
         mbar_wait(&ms.s_ready[kb & 1], (kb >> 1) & 1, wt, kSiteS, kb);
         tc_fence_after();
-        if (k + 1 == w.k1 && another) request_q(ahead.b);                 // all products with this piece's Q are complete
         float v[2][16];
         float mx[2] = {-INFINITY, -INFINITY};
         if (live) {
@@ -302,7 +290,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
             }
           }
           softmax_sync();
-          mbar_wait(&ms.pv_done[(kb - 1) & 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+          mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < 4 * kRows; c += 16) {
@@ -348,7 +336,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&ms.p_ready[kb & 1]);
       }
-      if (another) pass_q();
       // epilogue: O^T has dims on lanes; a warp writes 32 dims of a row at a time
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -370,187 +357,273 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
           }
         }
       softmax_sync();
-      mbar_wait(&ms.pv_done[(kb - 1) & 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+      mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
       tc_fence_after();
       const int rows = min(kRows, p.rows - rt * kRows);
+      float o[2][16];
+      tmem_ld16(tmem + lane_base, o[0]);
 #pragma unroll 1
-      for (int c = 0; c < 4 * kRows; c += 16) {
-        float o[16];
-        tmem_ld16(tmem + lane_base + c, o);
-        tmem_wait_ld();
-        const int r = c & (kRows - 1), d = c / kRows * 128 + 32 * warp + lane;
-        if (whole) {
-          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kRows + r) * kDV + d;
+      for (int c0 = 0; c0 < 4 * kRows; c0 += 32) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (r + e < rows) {
-              const float f = ms.corr[r + e];
-              dst[e * kDV] = __float2bfloat16(f > 0.f ? o[e] * f : 0.f);      // a row without keys: 0, whatever the values of others
-            }
-        } else {
-          float* dst = p.part_o + ((long long)slot * kRows + r) * kDV + d;
+        for (int u = 0; u < 2; ++u) {                                     // (the next columns come while these are written)
+          const int c = c0 + 16 * u, r = c & (kRows - 1), d = c / kRows * 128 + 32 * warp + lane;
+          tmem_wait_ld();
+          if (c + 16 < 4 * kRows) tmem_ld16(tmem + lane_base + c + 16, o[u ^ 1]);
+          if (whole) {
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kRows + r) * kDV + d;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (r + e < rows) dst[e * kDV] = o[e];
+            for (int e = 0; e < 16; ++e)
+              if (r + e < rows) {
+                const float f = ms.corr[r + e];
+                dst[e * kDV] = __float2bfloat16(f > 0.f ? o[u][e] * f : 0.f);      // a row without keys: 0, whatever the values of others
+              }
+          } else {
+            float* dst = p.part_o + ((long long)slot * kRows + r) * kDV + d;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (r + e < rows) dst[e * kDV] = o[u][e];
+          }
         }
       }
       tc_fence_before();
       w = ahead;
       more = another;
     }
-  } else if (warp == kWarpMma) {
-    // ------------------------------------------------------------ the two products (one thread)
+  } else if (warp == kWarpQk) {
+    // ------------------------------------------------------------ S = Q K^T (one thread)
+    // Two threads issue the products: with one, the second product of a block would wait behind the keys of the next.  S is free
+    // when a block's keys are there: its slot was given back by the second product of the block that had it, and the S, before.
     if (elect_one()) {
-      constexpr uint32_t idesc_qk = umma_idesc(1, 1, false, false, 64, kBlock);
-      constexpr uint32_t idesc_pv = umma_idesc(1, 1, true, false, 128, kRows);
+      constexpr uint32_t idesc = umma_idesc(1, 1, false, false, 64, kBlock);
       const uint64_t q_desc = umma_desc(sbase + PL::kOffQ, 16, 1024, kSwz128);
-      bool ok = true;
-      auto qk = [&](int kb) {
-        if (!(ok = mbar_wait(&ms.kv_full[kb & 1], (kb >> 1) & 1, wt, kSiteKv, kb))) return;
-        tc_fence_after();
-        const uint64_t kd = umma_desc(sbase + PL::kOffKV + (kb & 1) * kSlotBytes, 16, 1024, kSwz128);
-        const uint32_t d = tmem + PL::kTmemS + 64 * (kb & 1);
-#pragma unroll 1
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma_f16(d, q_desc + (PL::kQChunk >> 4) * j + 2 * s, kd + (kChunkBytes >> 4) * j + 2 * s, idesc_qk, (uint32_t)(j | s));
-        mma_commit_cta(&ms.s_ready[kb & 1]);
-      };
-      auto pv = [&](int kb, bool first) {
-        if (!(ok = mbar_wait(&ms.p_ready[kb & 1], (kb >> 1) & 1, wt, kSiteP, kb))) return;
-        tc_fence_after();
-        const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
-        const uint64_t vd = umma_desc(slot, kChunkBytes, 1024, kSwz128);                            // dims along M: two chunks of 64, 8 keys 1024 bytes
-        const uint64_t pd = umma_desc(slot + (kChunks - 1) * kChunkBytes, 16, 1024, kSwz128);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma_f16(tmem + kRows * i, vd + (2 * kChunkBytes >> 4) * i + 128 * s, pd + 2 * s, idesc_pv, first && s == 0 ? 0u : 1u);
-        mma_commit_cta(&ms.pv_done[kb & 1]);
-      };
       Walk w(ms);
-      int kb = 0, seg = 0;
-      bool first_before = false;                                          // whether block kb - 1 is its piece's first
-      for (; ok && w.next(p); ++seg) {
+      int kb = 0;
+      bool ok = true;
+      while (ok && w.next(p)) {
+        if (!(ok = mbar_wait(&ms.q_ready, w.index & 1, wt, kSiteQ, kb))) break;
         for (int k = w.k0; ok && k < w.k1; ++k, ++kb) {
-          const bool first = k == w.k0;
-          // the next piece's queries come in while its predecessor's last block is finished
-          if (first) {
-            if (kb > 0) pv(kb - 1, first_before);
-            if (ok) ok = mbar_wait(&ms.q_ready, seg & 1, wt, kSiteQ, kb);
-            if (ok) qk(kb);
-          } else {
-            qk(kb);
-            if (ok) pv(kb - 1, first_before);
+          const uint64_t kd = umma_desc(sbase + PL::kOffKV + (kb & 1) * kSlotBytes, 16, 1024, kSwz128);
+          const uint32_t d = tmem + PL::kTmemS + 64 * (kb & 1);
+#pragma unroll 1
+          for (int j = 0; j < kChunks; ++j) {
+            if ((j & 1) == 0) {
+              if (!(ok = mbar_wait(&ms.kv_full[kb & 1][j >> 1], (kb >> 1) & 1, wt, kSiteKv, kb))) break;
+              tc_fence_after();
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_f16(d, q_desc + (PL::kQChunk >> 4) * j + 2 * s, kd + (kChunkBytes >> 4) * j + 2 * s, idesc, (uint32_t)(j | s));
           }
-          first_before = first;
+          if (ok) mma_commit_cta(&ms.s_ready[kb & 1]);
         }
+        if (ok) mma_commit_cta(&ms.q_free);
       }
-      if (ok && kb > 0) pv(kb - 1, first_before);
       if (!ok) {                                                          // given up: what has been issued ends before the tensor memory goes
-        mma_commit_cta(&ms.drained);
-        mbar_drain(&ms.drained, 0);
+        mma_commit_cta(&ms.drained[0]);
+        mbar_drain(&ms.drained[0], 0);
       }
     }
     __syncwarp();
-  } else if (!kPacked) {
-    // ------------------------------------------------------------ bf16 rows by TMA
-    Walk w(ms);
-    int kb = 0, asked = 0;
-    bool ok = true;
-    const int boxes = kBlock / p.box_rows;                                // a box: rows of one page (at most 64), 64 dims
-    while (ok && w.next(p)) {
-      const int32_t* table = p.table + w.b * p.table_pitch;
-      for (int k = w.k0; k < w.k1; ++k, ++kb) {
-        int page = 0;                                                     // lane i: box i's page
-        const int at = k * kBlock + lane * p.box_rows;
-        const bool in = lane < boxes && at < w.len;
-        if (in) page = __ldcg(table + at / p.block_size);
-        const int n = __popc(__ballot_sync(0xffffffffu, in));
-        if (kb >= kSlots && !(ok = mbar_wait(&ms.pv_done[kb & 1], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb))) break;
-        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1], (uint32_t)(n * p.box_rows * kD * 2));
-        __syncwarp();
-        for (int i = 0; i < n; ++i) {
-          const int pg = __shfl_sync(0xffffffffu, page, i), row = (k * kBlock + i * p.box_rows) % p.block_size;
-          if (lane < kChunks)
-            tma_load_3d_hint(sbase + PL::kOffKV + (kb & 1) * kSlotBytes + lane * kChunkBytes + i * p.box_rows * 128, &map_kv, 64 * lane, row, pg,
-                             &ms.kv_full[kb & 1], l2_policy_evict_first());
+  } else if (warp == kWarpPv) {
+    // ------------------------------------------------------------ O^T += V^T P^T (one thread)
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc(1, 1, true, false, 128, kRows);
+      Walk w(ms);
+      int kb = 0;
+      bool ok = true;
+      while (ok && w.next(p))
+        for (int k = w.k0; k < w.k1; ++k, ++kb) {
+          if (!(ok = mbar_wait(&ms.p_ready[kb & 1], (kb >> 1) & 1, wt, kSiteP, kb))) break;
+          tc_fence_after();
+          const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+          const uint64_t vd = umma_desc(slot, kChunkBytes, 1024, kSwz128);                          // dims along M: two chunks of 64, 8 keys 1024 bytes
+          const uint64_t pd = umma_desc(slot + (kChunks - 1) * kChunkBytes, 16, 1024, kSwz128);
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_f16(tmem + kRows * i, vd + (2 * kChunkBytes >> 4) * i + 128 * s, pd + 2 * s, idesc, k == w.k0 && s == 0 ? 0u : 1u);
+            mma_commit_cta(&ms.kv_free[kb & 1][i]);
+          }
+          mma_commit_cta(&ms.kv_free[kb & 1][kGroups - 1]);
         }
-        asked = kb + 1;
+      if (!ok) {
+        mma_commit_cta(&ms.drained[1]);
+        mbar_drain(&ms.drained[1], 0);
       }
     }
-    if (!ok)
-      for (int i = max(asked - kSlots, 0); i < asked; ++i) mbar_drain(&ms.kv_full[i & 1], (i >> 1) & 1);
+    __syncwarp();
+  } else if (warp == kWarpQ) {
+    // ------------------------------------------------------------ queries of the next piece, when the last product with these is complete
+    Walk w(ms);
+    const uint64_t pol = l2_policy_evict_first();
+    bool ok = true;
+    int asked = 0;
+    while (w.next(p)) {
+      if (w.index > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.q_free, (w.index - 1) & 1, wt, kSiteQ, w.index)))) break;
+      if (p.flat_q) {
+        if (lane == 0) mbar_arrive_expect_tx(&ms.q_ready, kChunks * PL::kQChunk);
+        __syncwarp();
+        if (lane < kChunks) tma_load_3d_hint(sbase + PL::kOffQ + lane * PL::kQChunk, &map_q, 64 * lane, rt * kRows, w.b, &ms.q_ready, pol);
+      } else {
+        for (int r = 0; r < kRows; ++r) {
+          const int row = rt * kRows + r, j = row / p.heads, h = row - j * p.heads;
+          const bool in = row < p.rows;
+          const uint8_t* src = p.q + (in ? w.b * p.q_b + j * p.q_j + h * p.q_h : 0);
+          for (int c = lane; c < kD / 8; c += 32)
+            cp_async16_or_zero(sbase + PL::kOffQ + (uint32_t)(c >> 3) * PL::kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? 16 * c : 0), in);
+        }
+        cp_async_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.q_ready);
+      }
+      ++asked;
+    }
+    if (!ok && asked > 0 && lane == 0) mbar_drain(&ms.q_ready, (asked - 1) & 1);        // given up: what is in flight lands first
+    __syncwarp();
+  } else if (!kPacked) {
+    // ------------------------------------------------------------ bf16 rows by TMA
+    // A box: 64 dims of rows of one page, at most 64 of them.  A group's two chunks have a warp each (small boxes are paced by their
+    // issue), a lane a box.  Lane i keeps the page of box i of the blocks under way, of which the furthest, two ahead of the one
+    // requested, is brought into L2: the load that follows a freed slot then takes L2's latency.
+    struct Coming { int page, n, row; };                                  // n: boxes that hold keys (0: none of them does, or no block)
+    Walk w(ms);
+    const int count = ms.count;
+    int at = 0, looked = 0;
+    if (w.next(p)) at = w.k0;
+    auto look = [&]() -> Coming {
+      Coming c{-1, 0, 0};
+      if (looked >= count) return c;
+      const int key = at * kBlock + lane * p.box_rows;
+      const bool in = lane * p.box_rows < kBlock && key < w.len;
+      if (in) c.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
+      c.n = __popc(__ballot_sync(0xffffffffu, in));
+      c.row = key % p.block_size;
+      ++looked;
+      if (++at == w.k1 && w.next(p)) at = w.k0;
+      return c;
+    };
+    const uint64_t pol = l2_policy_evict_first();
+    const int half = warp - kWarpLoad0;
+    const uint32_t mine = sbase + PL::kOffKV + half * kChunkBytes + lane * p.box_rows * 128;
+    int asked = 0;
+    bool ok = true;
+    Coming c0 = look(), c1 = look(), c2 = look();
+    for (int kb = 0; ok && kb < count; ++kb) {
+      const Coming c3 = look();
+#pragma unroll 1
+      for (int j = 0; j < kGroups; ++j) {
+        if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
+        const bool has = j < kGroups - 1 || half == 0;
+        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1][j], has ? (uint32_t)(c0.n * p.box_rows * 128) : 0u);
+        __syncwarp();
+        if (lane < c0.n && has)
+          tma_load_3d_hint(mine + (kb & 1) * kSlotBytes + 2 * j * kChunkBytes, &map_kv, 64 * (2 * j + half), c0.row, c0.page, &ms.kv_full[kb & 1][j], pol);
+        asked = kGroups * kb + j + 1;
+      }
+      if (half == 1 && lane < c2.n && (unsigned)c2.page < (unsigned)p.n_blocks && (looked + rt) % p.row_tiles == 0)
+        l2_prefetch_1d(p.cache + (long long)c2.page * p.block_pitch + (long long)c2.row * (2 * kD), (uint32_t)(p.box_rows * 2 * kD));
+      c0 = c1; c1 = c2; c2 = c3;
+    }
+    if (!ok)                                                              // given up: what is in flight lands first
+      for (int i = max(asked - kSlots * kGroups, 0); i < asked; ++i) {
+        const int kb = i / kGroups;
+        mbar_drain(&ms.kv_full[kb & 1][i - kb * kGroups], (kb >> 1) & 1);
+      }
   } else {
     // ------------------------------------------------------------ packed rows through registers
-    // Warp v has rows v, v + 8, ..: a lane 16 codes of each, and 16 bytes of two rows' rope dims.
-    const int v = warp - kWarpLoad0;
-    uint4 codes[8], rope[2];
-    float scale[8];
-    auto row_at = [&](const Walk& w, int key) -> const uint8_t* {
-      const int page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
-      if ((unsigned)page >= (unsigned)p.n_blocks) return nullptr;
-      return p.cache + (long long)page * p.block_pitch + (long long)(key % p.block_size) * kPackedRow;
-    };
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    auto load = [&](const Walk& w, int k) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = k * kBlock + v + 8 * i;
-        const uint8_t* src = key < w.len ? row_at(w, key) : nullptr;
-        codes[i] = zero;
-        scale[i] = 0.f;
-        if (src) {
-          codes[i] = __ldcs(reinterpret_cast<const uint4*>(src) + lane);
-          scale[i] = __ldcg(reinterpret_cast<const float*>(src + 512) + (lane >> 3));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = k * kBlock + v + 8 * (4 * i + (lane >> 3));
-        const uint8_t* src = key < w.len ? row_at(w, key) : nullptr;
-        rope[i] = src ? __ldcs(reinterpret_cast<const uint4*>(src + 528) + (lane & 7)) : zero;
-      }
-    };
+    // Warp v has rows 8 v .. 8 v + 7 of a block (of one page: pages are multiples of 16 rows); of each 128 dims eight lanes have 16
+    // codes of a row each, four rows at a time.  A group's registers are loaded for the next block as soon as they are converted for this
+    // one, from L2, where the rows were brought a block before.
+    struct Coming { int page, row, n; };                                  // n of the warp's rows hold keys
+    const int v = warp - kWarpLoad0, sub = lane >> 3, c = lane & 7;
     Walk w(ms);
-    bool more = w.next(p);
-    int k = w.k0, kb = 0;
-    if (more) load(w, k);
-    while (more) {
-      if (kb >= kSlots && !mbar_wait(&ms.pv_done[kb & 1], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)) break;
-      const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = v + 8 * i;
-        uint4 a, b;
-        convert16(codes[i], scale[i], a, b);
-        // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
-        const uint32_t base = slot + (uint32_t)(lane >> 2) * kChunkBytes + r * 128;
-        const uint32_t u = 2 * (lane & 3), odd = (lane >> 2) & 1;
-        st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
-        st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
-      }
+    const int count = ms.count;
+    int at = 0, looked = 0;
+    if (w.next(p)) at = w.k0;
+    auto look = [&]() -> Coming {
+      Coming x{-1, 0, 0};
+      if (looked >= count) return x;
+      const int key = at * kBlock + 8 * v;
+      x.n = min(max(w.len - key, 0), 8);
+      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
+      x.row = key % p.block_size;
+      ++looked;
+      if (++at == w.k1 && w.next(p)) at = w.k0;
+      return x;
+    };
+    auto rows_of = [&](const Coming& x) -> const uint8_t* {
+      return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kPackedRow : nullptr;
+    };
+    uint4 codes[2 * (kGroups - 1)], rope[2];
+    float scale[2][kGroups - 1];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto load = [&](const uint8_t* src, int n, int j) {                    // group j's registers
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r = v + 8 * (4 * i + (lane >> 3));
-        st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), rope[i]);
+        const int r = sub + 4 * i;
+        const bool in = src != nullptr && r < n;
+        const uint8_t* row = src + r * kPackedRow;
+        if (j == 0) {
+          const float4 f = in ? __ldcg(reinterpret_cast<const float4*>(row + 512)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          scale[i][0] = f.x; scale[i][1] = f.y; scale[i][2] = f.z; scale[i][3] = f.w;
+        }
+        if (j < kGroups - 1) codes[(2 * j + i) % (2 * (kGroups - 1))] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 128 * j) + c) : zero;
+        else rope[i] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 528) + c) : zero;
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1]);
-      ++kb;
-      if (++k == w.k1) {
-        more = w.next(p);
-        k = w.k0;
+    };
+    auto to_l2 = [&](const Coming& x) {
+      const uint8_t* src = rows_of(x);
+      if (src != nullptr && lane == 0) l2_prefetch_1d(src, (uint32_t)(x.n * kPackedRow));
+    };
+    bool ok = true;
+    Coming c0 = look(), c1 = look(), c2 = look();
+    to_l2(c0);
+    to_l2(c1);
+    {
+      const uint8_t* src = rows_of(c0);
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) load(src, c0.n, j);
+    }
+    for (int kb = 0; ok && kb < count; ++kb) {
+      const Coming c3 = look();
+      const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+      const uint8_t* next = rows_of(c1);
+      if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
+      float mult[2][kGroups - 1];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kGroups - 1; ++j) mult[i][j] = scale[i][j];
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) {
+        if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = 8 * v + sub + 4 * i;
+          if (j < kGroups - 1) {
+            uint4 a, b;
+            convert16(codes[(2 * j + i) % (2 * (kGroups - 1))], mult[i][j % (kGroups - 1)], a, b);
+            // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
+            const uint32_t base = slot + (2 * j + (c >> 2)) * kChunkBytes + r * 128, u = 2 * (c & 3), odd = c >> 2;
+            st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
+            st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
+          } else {
+            st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + ((c ^ (r & 7)) << 4), rope[i]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1][j]);
+        load(next, c1.n, j);
       }
-      if (more) load(w, k);
+      c0 = c1; c1 = c2; c2 = c3;
     }
   }
 
   // which sequence of this group others have the rest of
-  if (warp == kWarpMma && rt == 0 && lane == 0 && p.meta) {
+  if (warp == kWarpQk && rt == 0 && lane == 0 && p.meta) {
     int4 e = make_int4(-1, 0, 0, 0);
     Walk w(ms);
     int before = 0;
@@ -566,7 +639,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const Params p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kWarpMma) tmem_dealloc_cta(tmem, PL::kTmemCols);
+  if (warp == kWarpQk) tmem_dealloc_cta(tmem, PL::kTmemCols);
   if (threadIdx.x == 0) {
     wt.report(g_status, p.epoch);
     if (blockIdx.x == 0) atomicAdd(&g_status[3], 1);
@@ -666,10 +739,10 @@ struct Shape {
 };
 
 template <int kRows, bool kPacked>
-static int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
+static int launch(const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
   if (!ensure_smem<mla_decode_kernel<kRows, kPacked>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
-  return launch_pdl(mla_decode_kernel<kRows, kPacked>, dim3((unsigned)(p.groups * p.row_tiles)), 32 * (kWarpLoad0 + (kPacked ? kPackedWarps : 1)),
-                    Plan<kRows>::kSmem, st, map, p);
+  return launch_pdl(mla_decode_kernel<kRows, kPacked>, dim3((unsigned)(p.groups * p.row_tiles)), 32 * (kWarpLoad0 + (kPacked ? kPackedWarps : kBf16Warps)),
+                    Plan<kRows>::kSmem, st, map, map_q, p);
 }
 
 }  // namespace decode
@@ -721,10 +794,17 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
       !make_map_3d(&map, cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)block_size, (uint64_t)n_blocks, 2 * kD,
                    (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, (uint32_t)p.box_rows, 1))
     return LITEDSA_ERR_CUDA;
+  // Rows (token, head) of a sequence that are evenly spaced (one token, or no gap behind a token's heads) are a matrix.
+  CUtensorMap map_q = {};
+  p.flat_q = q_len == 1 || q_token_stride == heads * q_head_stride;
+  const int64_t row_stride = heads > 1 ? q_head_stride : q_len > 1 ? q_token_stride : kD;
+  if (p.flat_q && !make_map_3d(&map_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)p.rows, (uint64_t)B, (uint64_t)(2 * row_stride),
+                               (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)s.per, 1))
+    p.flat_q = 0;                                                          // (a stride of 0, for one, is no map's)
   int rc;
-  if (s.per == 16) rc = packed ? launch<16, true>(map, p, st) : launch<16, false>(map, p, st);
-  else if (s.per == 32) rc = packed ? launch<32, true>(map, p, st) : launch<32, false>(map, p, st);
-  else rc = packed ? launch<64, true>(map, p, st) : launch<64, false>(map, p, st);
+  if (s.per == 16) rc = packed ? launch<16, true>(map, map_q, p, st) : launch<16, false>(map, map_q, p, st);
+  else if (s.per == 32) rc = packed ? launch<32, true>(map, map_q, p, st) : launch<32, false>(map, map_q, p, st);
+  else rc = packed ? launch<64, true>(map, map_q, p, st) : launch<64, false>(map, map_q, p, st);
   if (rc != LITEDSA_OK || s.groups == 1) return rc;
   return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)p.rows, (unsigned)min(B, s.groups)), 32 * kMergeWarps, 0, st, p, s.per);
 }
