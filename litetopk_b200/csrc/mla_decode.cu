@@ -34,7 +34,12 @@ constexpr uint32_t kChunkBytes = kBlock * 128;              // 64 keys x 64 bf16
 constexpr uint32_t kSlotBytes = kChunks * kChunkBytes;
 constexpr int kSlots = 2;
 constexpr int kGroups = 5;                                  // a tile's chunks are loaded and given back in groups: four of 128 dims, the rope dims
-constexpr int kWarpQk = 4, kWarpPv = 5, kWarpQ = 6, kWarpLoad0 = 7, kBf16Warps = 2, kPackedWarps = 8;
+// Warps 0-7: softmax.  Who loads: one warp by TMA (bf16 rows in pages of multiples of 64), 8 by cp.async (bf16 rows in smaller pages:
+// a box is a page then, and 36 boxes a block take a warp 3400 cycles to issue), 16 through registers (packed rows).
+enum Load { kTma, kCopy, kPacked };
+constexpr int kSoftmaxWarps = 8, kWarpQk = 8, kWarpPv = 9, kWarpQ = 10, kWarpTma = 11, kWarpLoad0 = 12;
+template <Load kLoad> constexpr int kLoadWarps = kLoad == kTma ? 0 : kLoad == kCopy ? 8 : 16;
+template <Load kLoad> constexpr int kThreads = 32 * (kWarpLoad0 + kLoadWarps<kLoad>);
 constexpr int kPackedRow = 656;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMInit = -1e30f;
@@ -60,8 +65,8 @@ struct Misc {
   uint32_t left, tmem_base;
   int start_b, start_k, count, meta_groups;
   long long start_pos, total;
-  int scan[16];
-  float corr[64];
+  int scan[32];
+  float corr[64], top[2][64], sum[2][64];
 };
 static_assert(sizeof(Misc) <= 2048, "Misc");
 
@@ -79,7 +84,7 @@ struct Params {
   float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
   int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
   int flat_q;                     // a sequence's rows are evenly spaced: they come by TMA
-  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows;
+  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks;
   float scale_log2;
   int epoch;
   uint32_t wait_limit;
@@ -97,10 +102,10 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool softmax_any(bool x) {
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                : "=r"(r) : "r"((uint32_t)x) : "memory");
   return r != 0;
 }
@@ -153,8 +158,8 @@ __device__ __forceinline__ void st_shared16(uint32_t a, const uint4& v) {
 }
 __device__ __forceinline__ void st_shared4(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 
-template <int kRows, bool kPacked>
-__global__ void __launch_bounds__(kPacked ? 32 * (kWarpLoad0 + kPackedWarps) : 32 * (kWarpLoad0 + kBf16Warps), 1)
+template <int kRows, Load kLoad>
+__global__ void __launch_bounds__(kThreads<kLoad>, 1)
 mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q, const Params p) {
   using PL = Plan<kRows>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -167,15 +172,15 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i)
-      for (int j = 0; j < kGroups; ++j) { mbar_init(&ms.kv_full[i][j], kPacked ? kPackedWarps : kBf16Warps); mbar_init(&ms.kv_free[i][j], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4); }
+      for (int j = 0; j < kGroups; ++j) { mbar_init(&ms.kv_full[i][j], kLoad == kTma ? 1 : kLoad == kCopy ? 32 * kLoadWarps<kCopy> : kLoadWarps<kPacked>); mbar_init(&ms.kv_free[i][j], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], kSoftmaxWarps); }
     mbar_init(&ms.q_ready, 1);
     mbar_init(&ms.q_free, 1);
     for (int i = 0; i < 2; ++i) mbar_init(&ms.drained[i], 1);
     ms.left = 0;
     ms.count = 0;
     fence_mbar_init();
-    if (!kPacked) tma_prefetch_desc(&map_kv);
+    if (kLoad == kTma) tma_prefetch_desc(&map_kv);
     if (p.flat_q) tma_prefetch_desc(&map_q);
   }
   if (warp == kWarpQk) {
@@ -220,15 +225,15 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
   }
   const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem_base, 0);
 
-  if (warp < 4) {
+  if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax, epilogue
-    // A warp has 16 rows: lane l rows l / 4 and l / 4 + 8, of every 8 keys the pair 2 (l % 4).
-    const int r0 = 16 * warp + (lane >> 2), qd = lane & 3;
-    const bool live = 16 * warp < kRows;
-    const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
+    // A warp has 16 rows and half of a block's keys: lane l rows l / 4 and l / 4 + 8, of every 8 keys the pair 2 (l % 4).
+    const int quarter = warp & 3, half = warp >> 2, r0 = 16 * quarter + (lane >> 2), qd = lane & 3;
+    const bool live = 16 * quarter < kRows;
+    const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
     Walk w(ms);
     int kb = 0;
-    // A wait here that gives up is passed like any other: the four warps meet at named barriers, so they take the same steps.
+    // A wait here that gives up is passed like any other: the warps meet at named barriers, so they take the same steps.
     bool more = w.next(p);
     while (more) {
       // rows' limits
@@ -240,95 +245,84 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       }
       low = w.len - p.q_len + 1 + rt * kRows / p.heads;                   // what the tile's first row sees
       float m[2] = {kMInit, kMInit}, l[2] = {0.f, 0.f};
-      Walk ahead = w;
-      const bool another = ahead.next(p);
       for (int k = w.k0; k < w.k1; ++k, ++kb) {
         mbar_wait(&ms.s_ready[kb & 1], (kb >> 1) & 1, wt, kSiteS, kb);
         tc_fence_after();
-        float v[2][16];
+        float v[16];
         float mx[2] = {-INFINITY, -INFINITY};
         if (live) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) tmem_ld_16x256b_x4(tmem + PL::kTmemS + 64 * (kb & 1) + 32 * c + lane_base, v[c]);
+          tmem_ld_16x256b_x4(tmem + PL::kTmemS + 64 * (kb & 1) + 32 * half + lane_base, v);
           tmem_wait_ld();
-          const int key0 = k * kBlock + 2 * qd;
           if ((k + 1) * kBlock > low) {
+            const int key0 = k * kBlock + 32 * half + 2 * qd;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int key = key0 + 32 * c + 8 * (e >> 2) + (e & 1);
-                v[c][e] = key < lim[(e >> 1) & 1] ? v[c][e] * p.scale_log2 : -INFINITY;
-              }
+            for (int e = 0; e < 16; ++e) v[e] = key0 + 8 * (e >> 2) + (e & 1) < lim[(e >> 1) & 1] ? v[e] * p.scale_log2 : -INFINITY;
           } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) v[c][e] *= p.scale_log2;
+            for (int e = 0; e < 16; ++e) v[e] *= p.scale_log2;
           }
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], v[c][e]);
+          for (int e = 0; e < 16; ++e) mx[(e >> 1) & 1] = fmaxf(mx[(e >> 1) & 1], v[e]);
+        }
+        const bool first = k == w.k0;
+        if (softmax_any(first || mx[0] > m[0] + kOvershoot || mx[1] > m[1] + kOvershoot)) {
+          // the rows' maxima over the block, and O relative to them
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            if (live && qd == 0) ms.top[half][r0 + 8 * i] = mx[i];
           }
-        }
-        if (k == w.k0) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) m[i] = fmaxf(m[i], mx[i]);
-        } else if (softmax_any(mx[0] > m[0] + kOvershoot || mx[1] > m[1] + kOvershoot)) {
+          softmax_sync();
           if (live) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const float now = fmaxf(m[i], mx[i]), f = fast_exp2(m[i] - now);
+              const float now = fmaxf(m[i], fmaxf(ms.top[0][r0 + 8 * i], ms.top[1][r0 + 8 * i])), f = fast_exp2(m[i] - now);
               m[i] = now;
               l[i] *= f;
-              if (qd == 0) ms.corr[r0 + 8 * i] = f;
+              if (half == 0 && qd == 0) ms.corr[r0 + 8 * i] = f;
             }
           }
-          softmax_sync();
-          mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
-          tc_fence_after();
+          if (!first) {
+            softmax_sync();
+            mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < 4 * kRows; c += 16) {
-            float o[16];
-            tmem_ld16(tmem + lane_base + c, o);
-            tmem_wait_ld();
+            for (int c = 2 * kRows * half; c < 2 * kRows * (half + 1); c += 16) {
+              float o[16];
+              tmem_ld16(tmem + lane_base + c, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] *= ms.corr[(c & (kRows - 1)) + e];
-            const uint32_t* r = reinterpret_cast<const uint32_t*>(o);
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                         ::"r"(tmem + lane_base + c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+              for (int e = 0; e < 16; ++e) o[e] *= ms.corr[(c & (kRows - 1)) + e];
+              const uint32_t* r = reinterpret_cast<const uint32_t*>(o);
+              asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                           ::"r"(tmem + lane_base + c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                             "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+            }
+            tmem_wait_st();
           }
-          tmem_wait_st();
         }
         const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
         if (live) {
           // P takes the place of the block's rope dims, which the first product was the last to read
           const uint32_t prow = slot + (kChunks - 1) * kChunkBytes + r0 * 128 + 4 * qd;
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int i = 0; i < 4; ++i) {
+            float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float e[4];
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                e[x] = fast_exp2(v[c][4 * i + x] - m[x >> 1]);
-                l[x >> 1] += e[x];
-              }
-              const uint32_t at = prow + (((4 * c + i) ^ (r0 & 7)) << 4);
-              st_shared4(at, bf16x2(e[0], e[1]));
-              st_shared4(at + 8 * 128, bf16x2(e[2], e[3]));
+            for (int x = 0; x < 4; ++x) {
+              e[x] = fast_exp2(v[4 * i + x] - m[x >> 1]);
+              l[x >> 1] += e[x];
             }
+            const uint32_t at = prow + (((4 * half + i) ^ (r0 & 7)) << 4);
+            st_shared4(at, bf16x2(e[0], e[1]));
+            st_shared4(at + 8 * 128, bf16x2(e[2], e[3]));
+          }
         }
         const int valid = w.len - k * kBlock;
         if (valid < kBlock) {                                             // value rows behind the end: nothing, whatever the page holds
           const int from = max(valid, 0);
-          for (int i = (int)threadIdx.x; i < (kBlock - from) * 64; i += 128)
+          for (int i = (int)threadIdx.x; i < (kBlock - from) * 64; i += 32 * kSoftmaxWarps)
             st_shared16(slot + (uint32_t)((i >> 3) & 7) * kChunkBytes + (from + (i >> 6)) * 128 + (i & 7) * 16, make_uint4(0, 0, 0, 0));
         }
         fence_proxy_async_smem();
@@ -336,24 +330,26 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(&ms.p_ready[kb & 1]);
       }
-      // epilogue: O^T has dims on lanes; a warp writes 32 dims of a row at a time
+      // epilogue: O^T has dims on lanes; a warp writes 32 dims of a row at a time, half of the columns
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (live && qd == 0) ms.sum[half][r0 + 8 * i] = l[i];
       }
       const bool whole = w.whole();
       const int slot = (int)blockIdx.x * 2 + (w.index == 0 ? 0 : 1);
-      softmax_sync();                                                     // corr of an earlier rescaling has been read
-      if (live && qd == 0)
+      softmax_sync();
+      if (live && half == 0 && qd == 0)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = r0 + 8 * i, row = rt * kRows + r;
-          ms.corr[r] = whole ? (l[i] > 0.f ? 1.f / l[i] : 0.f) : 1.f;
+          const float sum = ms.sum[0][r] + ms.sum[1][r];
+          ms.corr[r] = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
           if (whole) {
-            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = l[i] > 0.f ? (m[i] + __log2f(l[i])) * kLn2 : INFINITY;
+            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m[i] + __log2f(sum)) * kLn2 : INFINITY;
           } else {
-            p.part_ml[(long long)slot * kRows + r] = make_float2(m[i], l[i]);
+            p.part_ml[(long long)slot * kRows + r] = make_float2(m[i], sum);
           }
         }
       softmax_sync();
@@ -361,14 +357,14 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       tc_fence_after();
       const int rows = min(kRows, p.rows - rt * kRows);
       float o[2][16];
-      tmem_ld16(tmem + lane_base, o[0]);
+      tmem_ld16(tmem + lane_base + 2 * kRows * half, o[0]);
 #pragma unroll 1
-      for (int c0 = 0; c0 < 4 * kRows; c0 += 32) {
+      for (int c0 = 2 * kRows * half; c0 < 2 * kRows * (half + 1); c0 += 32) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {                                     // (the next columns come while these are written)
-          const int c = c0 + 16 * u, r = c & (kRows - 1), d = c / kRows * 128 + 32 * warp + lane;
+          const int c = c0 + 16 * u, r = c & (kRows - 1), d = c / kRows * 128 + 32 * quarter + lane;
           tmem_wait_ld();
-          if (c + 16 < 4 * kRows) tmem_ld16(tmem + lane_base + c + 16, o[u ^ 1]);
+          if (c + 16 < 2 * kRows * (half + 1)) tmem_ld16(tmem + lane_base + c + 16, o[u ^ 1]);
           if (whole) {
             __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kRows + r) * kDV + d;
 #pragma unroll
@@ -386,8 +382,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         }
       }
       tc_fence_before();
-      w = ahead;
-      more = another;
+      more = w.next(p);
     }
   } else if (warp == kWarpQk) {
     // ------------------------------------------------------------ S = Q K^T (one thread)
@@ -408,6 +403,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
           for (int j = 0; j < kChunks; ++j) {
             if ((j & 1) == 0) {
               if (!(ok = mbar_wait(&ms.kv_full[kb & 1][j >> 1], (kb >> 1) & 1, wt, kSiteKv, kb))) break;
+              if (kLoad == kCopy) fence_proxy_async_smem();               // what cp.async wrote, for the tensor core
               tc_fence_after();
             }
 #pragma unroll
@@ -434,6 +430,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       while (ok && w.next(p))
         for (int k = w.k0; k < w.k1; ++k, ++kb) {
           if (!(ok = mbar_wait(&ms.p_ready[kb & 1], (kb >> 1) & 1, wt, kSiteP, kb))) break;
+          if (kLoad == kCopy) fence_proxy_async_smem();
           tc_fence_after();
           const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
           const uint64_t vd = umma_desc(slot, kChunkBytes, 1024, kSwz128);                          // dims along M: two chunks of 64, 8 keys 1024 bytes
@@ -482,31 +479,31 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     }
     if (!ok && asked > 0 && lane == 0) mbar_drain(&ms.q_ready, (asked - 1) & 1);        // given up: what is in flight lands first
     __syncwarp();
-  } else if (!kPacked) {
-    // ------------------------------------------------------------ bf16 rows by TMA
-    // A box: 64 dims of rows of one page, at most 64 of them.  A group's two chunks have a warp each (small boxes are paced by their
-    // issue), a lane a box.  Lane i keeps the page of box i of the blocks under way, of which the furthest, two ahead of the one
-    // requested, is brought into L2: the load that follows a freed slot then takes L2's latency.
-    struct Coming { int page, n, row; };                                  // n: boxes that hold keys (0: none of them does, or no block)
+  } else if (kLoad == kTma) {
+   if (warp == kWarpTma) {
+    // ------------------------------------------------------------ bf16 rows by TMA: a block is of one page, nine boxes of 64 dims
+    // All lanes keep the pages of the blocks under way, of which the furthest, two ahead of the one requested, is brought into L2: the
+    // load that follows a freed slot then takes L2's latency.
+    struct Coming { int page, row; };                                     // page -1: no block, or one without keys
     Walk w(ms);
     const int count = ms.count;
     int at = 0, looked = 0;
     if (w.next(p)) at = w.k0;
     auto look = [&]() -> Coming {
-      Coming c{-1, 0, 0};
+      Coming c{-1, 0};
       if (looked >= count) return c;
-      const int key = at * kBlock + lane * p.box_rows;
-      const bool in = lane * p.box_rows < kBlock && key < w.len;
-      if (in) c.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
-      c.n = __popc(__ballot_sync(0xffffffffu, in));
+      const int key = at * kBlock;
       c.row = key % p.block_size;
+      if (key < w.len) {
+        c.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
+        if ((unsigned)c.page >= (unsigned)p.n_blocks) c.page = p.n_blocks;                        // beyond the cache: reads as zeros
+      }
       ++looked;
       if (++at == w.k1 && w.next(p)) at = w.k0;
       return c;
     };
     const uint64_t pol = l2_policy_evict_first();
-    const int half = warp - kWarpLoad0;
-    const uint32_t mine = sbase + PL::kOffKV + half * kChunkBytes + lane * p.box_rows * 128;
+    const uint32_t mine = sbase + PL::kOffKV + lane * kChunkBytes;
     int asked = 0;
     bool ok = true;
     Coming c0 = look(), c1 = look(), c2 = look();
@@ -515,15 +512,14 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
 #pragma unroll 1
       for (int j = 0; j < kGroups; ++j) {
         if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
-        const bool has = j < kGroups - 1 || half == 0;
-        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1][j], has ? (uint32_t)(c0.n * p.box_rows * 128) : 0u);
+        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1][j], c0.page >= 0 ? (j < kGroups - 1 ? 2 : 1) * kChunkBytes : 0u);
         __syncwarp();
-        if (lane < c0.n && has)
-          tma_load_3d_hint(mine + (kb & 1) * kSlotBytes + 2 * j * kChunkBytes, &map_kv, 64 * (2 * j + half), c0.row, c0.page, &ms.kv_full[kb & 1][j], pol);
+        if (c0.page >= 0 && (lane >> 1) == j && lane < kChunks)
+          tma_load_3d_hint(mine + (kb & 1) * kSlotBytes, &map_kv, 64 * lane, c0.row, c0.page, &ms.kv_full[kb & 1][j], pol);
         asked = kGroups * kb + j + 1;
       }
-      if (half == 1 && lane < c2.n && (unsigned)c2.page < (unsigned)p.n_blocks && (looked + rt) % p.row_tiles == 0)
-        l2_prefetch_1d(p.cache + (long long)c2.page * p.block_pitch + (long long)c2.row * (2 * kD), (uint32_t)(p.box_rows * 2 * kD));
+      if (lane == 0 && c2.page >= 0 && c2.page < p.n_blocks && (looked + rt) % p.row_tiles == 0)
+        l2_prefetch_1d(p.cache + (long long)c2.page * p.block_pitch + (long long)c2.row * (2 * kD), kBlock * 2 * kD);
       c0 = c1; c1 = c2; c2 = c3;
     }
     if (!ok)                                                              // given up: what is in flight lands first
@@ -531,13 +527,14 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         const int kb = i / kGroups;
         mbar_drain(&ms.kv_full[kb & 1][i - kb * kGroups], (kb >> 1) & 1);
       }
-  } else {
-    // ------------------------------------------------------------ packed rows through registers
-    // Warp v has rows 8 v .. 8 v + 7 of a block (of one page: pages are multiples of 16 rows); of each 128 dims eight lanes have 16
-    // codes of a row each, four rows at a time.  A group's registers are loaded for the next block as soon as they are converted for this
-    // one, from L2, where the rows were brought a block before.
+   }
+  } else if (warp >= kWarpLoad0) {
+    // ------------------------------------------------------------ rows by cp.async, or packed rows through registers
+    // Warp v has kOwn adjacent rows of a block (of one page: pages are multiples of 16 rows).
+    constexpr int kOwn = kBlock / (kLoad == kTma ? 16 : kLoadWarps<kLoad>);
+    constexpr int kRowBytes = kLoad == kCopy ? 2 * kD : kPackedRow;
     struct Coming { int page, row, n; };                                  // n of the warp's rows hold keys
-    const int v = warp - kWarpLoad0, sub = lane >> 3, c = lane & 7;
+    const int v = warp - kWarpLoad0;
     Walk w(ms);
     const int count = ms.count;
     int at = 0, looked = 0;
@@ -545,8 +542,8 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     auto look = [&]() -> Coming {
       Coming x{-1, 0, 0};
       if (looked >= count) return x;
-      const int key = at * kBlock + 8 * v;
-      x.n = min(max(w.len - key, 0), 8);
+      const int key = at * kBlock + kOwn * v;
+      x.n = min(max(w.len - key, 0), kOwn);
       if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
       x.row = key % p.block_size;
       ++looked;
@@ -554,71 +551,95 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       return x;
     };
     auto rows_of = [&](const Coming& x) -> const uint8_t* {
-      return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kPackedRow : nullptr;
-    };
-    uint4 codes[2 * (kGroups - 1)], rope[2];
-    float scale[2][kGroups - 1];
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    auto load = [&](const uint8_t* src, int n, int j) {                    // group j's registers
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = sub + 4 * i;
-        const bool in = src != nullptr && r < n;
-        const uint8_t* row = src + r * kPackedRow;
-        if (j == 0) {
-          const float4 f = in ? __ldcg(reinterpret_cast<const float4*>(row + 512)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          scale[i][0] = f.x; scale[i][1] = f.y; scale[i][2] = f.z; scale[i][3] = f.w;
-        }
-        if (j < kGroups - 1) codes[(2 * j + i) % (2 * (kGroups - 1))] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 128 * j) + c) : zero;
-        else rope[i] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 528) + c) : zero;
-      }
+      return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kRowBytes : nullptr;
     };
     auto to_l2 = [&](const Coming& x) {
       const uint8_t* src = rows_of(x);
-      if (src != nullptr && lane == 0) l2_prefetch_1d(src, (uint32_t)(x.n * kPackedRow));
+      if (src != nullptr && lane == 0) l2_prefetch_1d(src, (uint32_t)(x.n * kRowBytes));
     };
     bool ok = true;
     Coming c0 = look(), c1 = look(), c2 = look();
     to_l2(c0);
     to_l2(c1);
-    {
-      const uint8_t* src = rows_of(c0);
+    if (kLoad == kCopy) {
+      for (int kb = 0; ok && kb < count; ++kb) {
+        const Coming c3 = look();
+        const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+        const uint8_t* src = rows_of(c0);
+        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) load(src, c0.n, j);
-    }
-    for (int kb = 0; ok && kb < count; ++kb) {
-      const Coming c3 = look();
-      const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
-      const uint8_t* next = rows_of(c1);
-      if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
-      float mult[2][kGroups - 1];
+        for (int j = 0; j < kGroups; ++j) {
+          if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
+          constexpr int kWide = 16;                                       // 16-byte pieces of a row in a group of two chunks
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kGroups - 1; ++j) mult[i][j] = scale[i][j];
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j) {
-        if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = 8 * v + sub + 4 * i;
-          if (j < kGroups - 1) {
-            uint4 a, b;
-            convert16(codes[(2 * j + i) % (2 * (kGroups - 1))], mult[i][j % (kGroups - 1)], a, b);
-            // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
-            const uint32_t base = slot + (2 * j + (c >> 2)) * kChunkBytes + r * 128, u = 2 * (c & 3), odd = c >> 2;
-            st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
-            st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
-          } else {
-            st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + ((c ^ (r & 7)) << 4), rope[i]);
+          for (int i = 0; i < (j < kGroups - 1 ? kOwn * kWide / 32 : kOwn * kWide / 64); ++i) {
+            const int x = lane + 32 * i, r = j < kGroups - 1 ? x / kWide : x / 8, c = j < kGroups - 1 ? x % kWide : x % 8;
+            const bool in = src != nullptr && r < c0.n;
+            const int row = kOwn * v + r;
+            cp_async16_or_zero(slot + (2 * j + (c >> 3)) * kChunkBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                               in ? src + r * kRowBytes + 256 * j + 16 * c : p.cache, in);
           }
+          cp_async_mbar_arrive_noinc(&ms.kv_full[kb & 1][j]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1][j]);
-        load(next, c1.n, j);
+        c0 = c1; c1 = c2; c2 = c3;
       }
-      c0 = c1; c1 = c2; c2 = c3;
+      cp_async_wait_all();
+    } else {
+      // Of each 128 dims eight lanes have 16 codes of a row each, four rows at a time.  A group's registers are loaded for the next
+      // block as soon as they are converted for this one, from L2, where the rows were brought a block before.
+      constexpr int kSets = kOwn / 4;
+      const int sub = lane >> 3, c = lane & 7;
+      uint4 codes[kGroups - 1][kSets], rope[kSets];
+      float4 scale[kSets];
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      auto load = [&](const uint8_t* src, int n, int j) {                  // group j's registers
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) {
+          const int r = sub + 4 * i;
+          const bool in = src != nullptr && r < n;
+          const uint8_t* row = src + r * kRowBytes;
+          if (j == 0) scale[i] = in ? __ldcg(reinterpret_cast<const float4*>(row + 512)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (j < kGroups - 1) codes[j % (kGroups - 1)][i] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 128 * j) + c) : zero;
+          else rope[i] = in ? __ldcg(reinterpret_cast<const uint4*>(row + 528) + c) : zero;
+        }
+      };
+      {
+        const uint8_t* src = rows_of(c0);
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) load(src, c0.n, j);
+      }
+      for (int kb = 0; ok && kb < count; ++kb) {
+        const Coming c3 = look();
+        const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
+        const uint8_t* next = rows_of(c1);
+        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
+        float4 mult[kSets];
+#pragma unroll
+        for (int i = 0; i < kSets; ++i) mult[i] = scale[i];
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+          if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
+#pragma unroll
+          for (int i = 0; i < kSets; ++i) {
+            const int r = kOwn * v + sub + 4 * i;
+            if (j < kGroups - 1) {
+              uint4 a, b;
+              convert16(codes[j % (kGroups - 1)][i], j == 0 ? mult[i].x : j == 1 ? mult[i].y : j == 2 ? mult[i].z : mult[i].w, a, b);
+              // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
+              const uint32_t base = slot + (2 * j + (c >> 2)) * kChunkBytes + r * 128, u = 2 * (c & 3), odd = c >> 2;
+              st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
+              st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
+            } else {
+              st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + ((c ^ (r & 7)) << 4), rope[i]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1][j]);
+          load(next, c1.n, j);
+        }
+        c0 = c1; c1 = c2; c2 = c3;
+      }
     }
   }
 
@@ -646,50 +667,23 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
   }
 }
 
-// The parts of row blockIdx.x of the blockIdx.y-th sequence that several groups have: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.
-// A warp sums every eighth part, all loads of four parts under way; the eight sums meet in shared memory.
-constexpr int kMergeWarps = 8;
-__global__ void __launch_bounds__(32 * kMergeWarps) mla_decode_merge_kernel(const Params p, int kRows) {
-  __shared__ float4 acc[kMergeWarps][kDV / 4];
-  __shared__ float sum_l[kMergeWarps];
-  __shared__ int pick[2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  pdl_trigger();
-  pdl_wait();
-  if (warp == 0) {                                   // the blockIdx.y-th entry of the list
-    int seen = 0, found = -1;
-    for (int g0 = 0; g0 < p.groups && found < 0; g0 += 32) {
-      const bool is = g0 + lane < p.groups && __ldcg(&p.meta[g0 + lane].x) >= 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, is);
-      const int want = (int)blockIdx.y - seen;
-      if (want < __popc(mask)) found = g0 + (int)__fns(mask, 0, want + 1);
-      seen += __popc(mask);
-    }
-    if (lane == 0) pick[0] = found;
-  }
-  __syncthreads();
-  const int g = pick[0];
-  if (g < 0) return;
-  const int4 e = __ldcg(p.meta + g);
-  const int row = (int)blockIdx.x, rt = row / kRows, r = row - rt * kRows, parts = e.z;
-  auto slot_of = [&](int i) -> long long { return ((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r; };
-  float m = kMInit;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(&p.part_ml[slot_of(i)].x));
+// The rows of sequences that several groups have parts of: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.  Blocks deal out the
+// rows among themselves: of a sequence of up to 8 parts a warp has a row, of one of more a block has: each warp sums every eighth
+// part and the eight sums meet in shared memory.  (With a block per row and listed sequence, mostly idle, 36 sequences of 256 rows in
+// two or three parts took 76 us.)
+constexpr int kMergeWarps = 8, kMaxGroups = 1024;      // (at most one a CTA)
+__device__ __forceinline__ void add_parts(const Params& p, int kRows, int g, const int4& e, int row, float m, int from, int step, float4 (&a)[4], float& l,
+                                          int lane) {
+  const int rt = row / kRows, r = row - rt * kRows;
+  for (int i0 = from; i0 < e.z; i0 += 2 * step) {
+    float4 v[2][4];
+    float2 ml[2];
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  float4 a[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int i0 = warp; i0 < parts; i0 += 4 * kMergeWarps) {
-    float4 v[4][4];
-    float2 ml[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kMergeWarps;
+    for (int u = 0; u < 2; ++u) {
+      const int i = i0 + u * step;
       ml[u] = make_float2(kMInit, 0.f);
-      if (i < parts) {
-        const long long s = slot_of(i);
+      if (i < e.z) {
+        const long long s = ((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r;
         ml[u] = __ldcg(&p.part_ml[s]);
         const float4* src = reinterpret_cast<const float4*>(p.part_o + s * kDV);
 #pragma unroll
@@ -697,8 +691,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_decode_merge_kernel(cons
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (!(ml[u].y > 0.f)) continue;                // beyond the list, or a part without keys
+    for (int u = 0; u < 2; ++u) {
+      if (!(ml[u].y > 0.f)) continue;                  // beyond the list, or a part without keys
       const float f = fast_exp2(ml[u].x - m);
       l += f * ml[u].y;
 #pragma unroll
@@ -707,23 +701,86 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_decode_merge_kernel(cons
       }
     }
   }
+}
+__global__ void __launch_bounds__(32 * kMergeWarps, 3) mla_decode_merge_kernel(const Params p, int kRows) {
+  __shared__ float4 acc[kMergeWarps][kDV / 4];
+  __shared__ float sum_l[kMergeWarps];
+  __shared__ int list[kMaxGroups], units[kMaxGroups + 1], n_list;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_trigger();
+  pdl_wait();
+  if (warp == 0) {                                     // the cut sequences, and where each one's units of work begin
+    int n = 0, u = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int parts = g0 + lane < p.groups && __ldcg(&p.meta[g0 + lane].x) >= 0 ? __ldcg(&p.meta[g0 + lane].z) : 0;
+      const uint32_t mask = __ballot_sync(0xffffffffu, parts > 0);
+      const int mine = parts == 0 ? 0 : parts <= 8 ? (p.rows + kMergeWarps - 1) / kMergeWarps : p.rows;
+      int incl = mine;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) acc[warp][32 * c + lane] = a[c];
-  if (lane == 0) sum_l[warp] = l;
-  __syncthreads();
-  if (threadIdx.x >= kDV / 4) return;
-  float4 o = acc[0][threadIdx.x];
-  l = sum_l[0];
-#pragma unroll
-  for (int w = 1; w < kMergeWarps; ++w) {
-    const float4 x = acc[w][threadIdx.x];
-    o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-    l += sum_l[w];
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      if (parts > 0) {
+        const int at = n + __popc(mask & ((1u << lane) - 1u));
+        list[at] = g0 + lane;
+        units[at] = u + incl - mine;
+      }
+      n += __popc(mask);
+      u += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) { units[n] = u; n_list = n; }
   }
-  const float f = l > 0.f ? 1.f / l : 0.f;
-  const long long at = (long long)e.x * p.rows + row;
-  reinterpret_cast<uint2*>(p.out)[at * (kDV / 4) + threadIdx.x] = make_uint2(bf16x2(o.x * f, o.y * f), bf16x2(o.z * f, o.w * f));      // (all parts without keys: o = 0)
-  if (threadIdx.x == 0) p.lse[at] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+  __syncthreads();
+  const int n = n_list, all = units[n];
+  int at = 0;
+  for (int u = (int)blockIdx.x; u < all; u += (int)gridDim.x) {
+    while (units[at + 1] <= u) ++at;
+    const int g = list[at];
+    const int4 e = __ldcg(p.meta + g);
+    const bool alone = e.z <= 8;                       // a warp a row
+    const int row = alone ? (u - units[at]) * kMergeWarps + warp : u - units[at];
+    if (row < p.rows) {                                // (the same for all of a block that shares a row)
+      const int rt = row / kRows, r = row - rt * kRows;
+      float m = kMInit;
+      for (int i = lane; i < e.z; i += 32)
+        m = fmaxf(m, __ldcg(&p.part_ml[((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r].x));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      float4 a[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+      add_parts(p, kRows, g, e, row, m, alone ? 0 : warp, alone ? 1 : kMergeWarps, a, l, lane);
+      const long long to = (long long)e.x * p.rows + row;
+      if (alone) {
+        const float f = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          reinterpret_cast<uint2*>(p.out)[to * (kDV / 4) + 32 * c + lane] = make_uint2(bf16x2(a[c].x * f, a[c].y * f), bf16x2(a[c].z * f, a[c].w * f));
+        if (lane == 0) p.lse[to] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[warp][32 * c + lane] = a[c];
+        if (lane == 0) sum_l[warp] = l;
+        __syncthreads();
+        if (threadIdx.x < kDV / 4) {
+          float4 o = acc[0][threadIdx.x];
+          l = sum_l[0];
+#pragma unroll
+          for (int w = 1; w < kMergeWarps; ++w) {
+            const float4 x = acc[w][threadIdx.x];
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+            l += sum_l[w];
+          }
+          const float f = l > 0.f ? 1.f / l : 0.f;
+          reinterpret_cast<uint2*>(p.out)[to * (kDV / 4) + threadIdx.x] = make_uint2(bf16x2(o.x * f, o.y * f), bf16x2(o.z * f, o.w * f));
+          if (threadIdx.x == 0) p.lse[to] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+        }
+        __syncthreads();
+      }
+    }
+  }
 }
 
 static int rows_per_cta(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
@@ -732,17 +789,21 @@ struct Shape {
   Shape(int rows) {
     per = rows_per_cta(rows);
     tiles = (rows + per - 1) / per;
-    groups = max(1, sm_count() / tiles);
+    groups = min(max(1, sm_count() / tiles), 1024);
   }
   int64_t part_bytes() const { return (int64_t)groups * tiles * 2 * per * (kDV * 4 + 8); }
   int64_t bytes() const { return groups == 1 ? 0 : part_bytes() + (int64_t)groups * 16; }
 };
 
-template <int kRows, bool kPacked>
+template <int kRows, Load kLoad>
 static int launch(const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
-  if (!ensure_smem<mla_decode_kernel<kRows, kPacked>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
-  return launch_pdl(mla_decode_kernel<kRows, kPacked>, dim3((unsigned)(p.groups * p.row_tiles)), 32 * (kWarpLoad0 + (kPacked ? kPackedWarps : kBf16Warps)),
-                    Plan<kRows>::kSmem, st, map, map_q, p);
+  if (!ensure_smem<mla_decode_kernel<kRows, kLoad>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
+  return launch_pdl(mla_decode_kernel<kRows, kLoad>, dim3((unsigned)(p.groups * p.row_tiles)), kThreads<kLoad>, Plan<kRows>::kSmem, st, map, map_q, p);
+}
+template <int kRows>
+static int launch(Load l, const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
+  return l == kTma ? launch<kRows, kTma>(map, map_q, p, st) : l == kCopy ? launch<kRows, kCopy>(map, map_q, p, st)
+                                                                         : launch<kRows, kPacked>(map, map_q, p, st);
 }
 
 }  // namespace decode
@@ -786,13 +847,13 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   }
   p.B = B; p.q_len = q_len; p.heads = heads; p.rows = q_len * heads; p.row_tiles = s.tiles; p.groups = s.groups;
   p.cols = n_blocks == 0 ? 0 : table_cols; p.block_size = block_size; p.n_blocks = (int)n_blocks;
-  p.box_rows = block_size % 64 == 0 ? 64 : block_size % 32 == 0 ? 32 : 16;
   p.scale_log2 = sm_scale * kLog2e;
   p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
   CUtensorMap map = {};
-  if (!packed && n_blocks > 0 &&
+  const Load load = packed ? kPacked : block_size % kBlock == 0 ? kTma : kCopy;
+  if (load == kTma && n_blocks > 0 &&
       !make_map_3d(&map, cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)block_size, (uint64_t)n_blocks, 2 * kD,
-                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, (uint32_t)p.box_rows, 1))
+                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, kBlock, 1))
     return LITEDSA_ERR_CUDA;
   // Rows (token, head) of a sequence that are evenly spaced (one token, or no gap behind a token's heads) are a matrix.
   CUtensorMap map_q = {};
@@ -801,12 +862,10 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   if (p.flat_q && !make_map_3d(&map_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)p.rows, (uint64_t)B, (uint64_t)(2 * row_stride),
                                (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)s.per, 1))
     p.flat_q = 0;                                                          // (a stride of 0, for one, is no map's)
-  int rc;
-  if (s.per == 16) rc = packed ? launch<16, true>(map, map_q, p, st) : launch<16, false>(map, map_q, p, st);
-  else if (s.per == 32) rc = packed ? launch<32, true>(map, map_q, p, st) : launch<32, false>(map, map_q, p, st);
-  else rc = packed ? launch<64, true>(map, map_q, p, st) : launch<64, false>(map, map_q, p, st);
+  const int rc = s.per == 16 ? launch<16>(load, map, map_q, p, st) : s.per == 32 ? launch<32>(load, map, map_q, p, st) : launch<64>(load, map, map_q, p, st);
   if (rc != LITEDSA_OK || s.groups == 1) return rc;
-  return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)p.rows, (unsigned)min(B, s.groups)), 32 * kMergeWarps, 0, st, p, s.per);
+  const int64_t most = (int64_t)min(B, s.groups) * p.rows;                 // rows that can need it
+  return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)min(most, (int64_t)3 * sm_count())), 32 * kMergeWarps, 0, st, p, s.per);
 }
 
 // Status block of the kernel; layout and return rule as litedsa_attn_status.
