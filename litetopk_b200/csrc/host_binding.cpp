@@ -1,11 +1,11 @@
-// The plain calls of sparse_prefill, lite_topk and the two DSv4 operators in one step from Python: arguments, output and workspace
+// The plain calls of sparse_prefill, lite_topk, the two DSv4 operators and those of dense.py in one step from Python: arguments, output and workspace
 // tensors, the C ABI.  A call of a few tokens takes 13 to 20 us on the device; by way of ctypes, with the checks and allocations in
 // Python, its host side took as long or longer and was what such calls were bound by: sparse_prefill of 2 tokens 22 us (11 this
 // way), dsv4_c128a_bf16 of 24 tokens 19 (9), lite_topk and sparse_prefill of 36 tokens 48 (19).
 //
-// Each function takes the arguments of its operator in api.py and returns the result (True from dsv4_masked_mla_bf16_out, whose caller
-// has it), the status code of a call that the library refused (lite_topk, which makes two: with the refused one's name), or None for
-// whatever is not plain: then nothing has been done, and api.py goes its own way, checks and errors included.  Plain are dense CUDA tensors of the expected types, shapes and strides on the current device that
+// Each function takes the arguments of its operator in api.py or dense.py and returns the result (True from dsv4_masked_mla_bf16_out and
+// append_kv, whose callers have it), the status code of a call that the library refused (lite_topk, which makes two: with the refused one's name), or None for
+// whatever is not plain: then nothing has been done, and the caller goes its own way, checks and errors included.  Plain are dense CUDA tensors of the expected types, shapes and strides on the current device that
 // no dispatch mode, function transform or subclass stands behind.
 #include <Python.h>
 
@@ -239,11 +239,148 @@ PyObject* lite_topk(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
+// A paged cache as dense.py takes it: [blocks, block_size, 576] bf16 or [blocks, block_size, 656] bytes, rows of a block dense
+bool paged(const Tensor& t, bool* packed, int64_t* pitch) {
+  *packed = t.scalar_type() == at::kByte;
+  const int64_t width = *packed ? 656 : 576;
+  if ((!*packed && t.scalar_type() != at::kBFloat16) || t.dim() != 3 || t.size(2) != width || t.stride(2) != 1 || t.size(0) <= 0 || t.size(1) <= 0 ||
+      !small(t.size(0)) || !small(t.size(1)) || (t.size(1) > 1 && t.stride(1) != width))
+    return false;
+  *pitch = t.stride(0) * (*packed ? 1 : 2);
+  return true;
+}
+
+// (kv_c, k_rope, positions, cos_sin, slots, kv_cache, interleaved, q_rope, q_out, k_out); True if done
+PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int dev = current_device(a[0]);
+    const Tensor *c = plain(a[0], dev), *k = plain(a[1], dev), *pos = plain(a[2], dev), *cs = plain(a[3], dev), *slots = plain(a[4], dev),
+                 *cache = plain(a[5], dev), *q = a[7] == Py_None ? nullptr : plain(a[7], dev), *qo = a[8] == Py_None ? nullptr : plain(a[8], dev),
+                 *ko = a[9] == Py_None ? nullptr : plain(a[9], dev);
+    bool packed = false;
+    int64_t pitch = 0;
+    if (!c || !k || !pos || !cs || !slots || !cache || !PyBool_Check(a[6]) || (a[7] != Py_None && !q) || (a[8] != Py_None && !qo) ||
+        (a[9] != Py_None && !ko) || (q == nullptr) != (qo == nullptr) || !paged(*cache, &packed, &pitch))
+      Py_RETURN_NONE;
+    const int64_t T = c->size(0);
+    auto rows = [&](const Tensor& t, int64_t d) {
+      return t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(0) == T && t.size(1) == d && t.stride(1) == 1;
+    };
+    auto index = [&](const Tensor& t) { return is_index(t) && t.dim() == 1 && t.size(0) == T && t.is_contiguous(); };
+    if (c->dim() != 2 || T <= 0 || !small(T) || !rows(*c, 512) || !rows(*k, 64) || (ko && !rows(*ko, 64)) || !index(*pos) || !index(*slots) ||
+        cs->dim() != 2 || cs->scalar_type() != at::kFloat || cs->size(1) != 64 || cs->stride(1) != 1 || cs->size(0) <= 0)
+      Py_RETURN_NONE;
+    int64_t heads = 0;
+    if (q) {
+      auto turned = [&](const Tensor& t) {
+        return t.dim() == 3 && t.scalar_type() == at::kBFloat16 && t.size(0) == T && t.size(1) == heads && t.size(2) == 64 && t.stride(2) == 1;
+      };
+      heads = q->dim() == 3 ? q->size(1) : 0;
+      if (heads <= 0 || !small(heads) || !turned(*q) || !turned(*qo)) Py_RETURN_NONE;
+    }
+    int rc;
+    {
+      NoGil unlocked;
+      rc = litedsa_append_kv(c->data_ptr(), c->stride(0), k->data_ptr(), k->stride(0), pos->data_ptr(), pos->scalar_type() == at::kLong,
+                             static_cast<const float*>(cs->data_ptr()), cs->size(0), cs->stride(0), slots->data_ptr(),
+                             slots->scalar_type() == at::kLong, cache->data_ptr(), packed, cache->size(0), (int)cache->size(1), pitch,
+                             a[6] == Py_True, q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, qo ? qo->data_ptr() : nullptr,
+                             qo ? qo->stride(0) : 0, qo ? qo->stride(1) : 0, (int)heads, ko ? ko->data_ptr() : nullptr, ko ? ko->stride(0) : 0, (int)T,
+                             stream_of(dev));
+    }
+    if (rc != LITEDSA_OK) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// (q, kv_cache, block_table, seq_lens, sm_scale)
+PyObject* mla_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int dev = current_device(a[0]);
+    const Tensor *q = plain(a[0], dev), *cache = plain(a[1], dev), *table = plain(a[2], dev), *lens = plain(a[3], dev);
+    double sm = 0;
+    bool packed = false;
+    int64_t pitch = 0;
+    if (!q || !cache || !table || !lens || !number(a[4], &sm) || !paged(*cache, &packed, &pitch) || cache->size(1) % 16 != 0) Py_RETURN_NONE;
+    const int64_t nd = q->dim();
+    if ((nd != 3 && nd != 4) || q->scalar_type() != at::kBFloat16 || q->size(-1) != 576 || q->stride(-1) != 1) Py_RETURN_NONE;
+    const int64_t B = q->size(0), q_len = nd == 4 ? q->size(1) : 1, heads = q->size(-2);
+    if (B <= 0 || !small(B) || q_len <= 0 || q_len > (1 << 20) || heads <= 0 || heads > 128 || table->dim() != 2 || table->scalar_type() != at::kInt ||
+        table->size(0) != B || table->size(1) <= 0 || !small(table->size(1)) || table->stride(1) != 1 || lens->dim() != 1 ||
+        lens->scalar_type() != at::kInt || lens->size(0) != B || !lens->is_contiguous())
+      Py_RETURN_NONE;
+    Tensor out, lse;
+    int rc;
+    {
+      NoGil unlocked;
+      out = nd == 4 ? empty({B, q_len, heads, 512}, at::kBFloat16, *q) : empty({B, heads, 512}, at::kBFloat16, *q);
+      lse = nd == 4 ? empty({B, q_len, heads}, at::kFloat, *q) : empty({B, heads}, at::kFloat, *q);
+      const int64_t bytes = litedsa_mla_decode_workspace((int)q_len, (int)heads);
+      Tensor ws = empty({bytes > 0 ? bytes : 1}, at::kByte, *q);
+      rc = litedsa_mla_decode(q->data_ptr(), q->stride(0), nd == 4 ? q->stride(1) : 0, q->stride(-2), cache->data_ptr(), packed, cache->size(0),
+                              (int)cache->size(1), pitch, static_cast<const int32_t*>(table->data_ptr()), table->stride(0), (int)table->size(1),
+                              static_cast<const int32_t*>(lens->data_ptr()), (float)sm, out.data_ptr(), static_cast<float*>(lse.data_ptr()), (int)B,
+                              (int)q_len, (int)heads, ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    return rc == LITEDSA_OK ? pair(out, lse) : PyLong_FromLong(rc);
+  });
+}
+
+// (q, k_nope, k_rope, v, sm_scale, cu_seqlens_q, cu_seqlens_k, causal)
+PyObject* mla_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) Py_RETURN_NONE;
+  return guarded([&]() -> PyObject* {
+    const int dev = current_device(a[0]);
+    const Tensor *q = plain(a[0], dev), *kn = plain(a[1], dev), *kr = plain(a[2], dev), *v = plain(a[3], dev),
+                 *cq = a[5] == Py_None ? nullptr : plain(a[5], dev), *ck = a[6] == Py_None ? nullptr : plain(a[6], dev);
+    double sm = 0;
+    if (!q || !kn || !kr || !v || !number(a[4], &sm) || !(sm >= 0) || (a[5] != Py_None && !cq) || (a[6] != Py_None && !ck) ||
+        (cq == nullptr) != (ck == nullptr) || !PyBool_Check(a[7]) || q->dim() != 3 || kr->dim() != 2)
+      Py_RETURN_NONE;
+    const int64_t Tq = q->size(0), heads = q->size(1), Tk = kr->size(0);
+    auto per_head = [&](const Tensor& t, int64_t rows, int64_t d) {
+      return t.dim() == 3 && t.scalar_type() == at::kBFloat16 && t.size(0) == rows && t.size(1) == heads && t.size(2) == d && t.stride(2) == 1;
+    };
+    if (Tq <= 0 || Tk <= 0 || heads <= 0 || !small(Tq) || !small(Tk) || !small(heads) || !per_head(*q, Tq, 192) || !per_head(*kn, Tk, 128) ||
+        !per_head(*v, Tk, 128) || kr->scalar_type() != at::kBFloat16 || kr->size(1) != 64 || kr->stride(1) != 1)
+      Py_RETURN_NONE;
+    int64_t B = 1;
+    if (cq) {
+      for (const Tensor* t : {cq, ck})
+        if (t->dim() != 1 || t->scalar_type() != at::kInt || t->size(0) != cq->size(0) || !t->is_contiguous()) Py_RETURN_NONE;
+      B = cq->size(0) - 1;
+      if (B <= 0 || !small(B)) Py_RETURN_NONE;
+    }
+    auto ints = [](const Tensor* t) { return t ? static_cast<const int32_t*>(t->data_ptr()) : nullptr; };
+    Tensor out, lse;
+    int rc;
+    {
+      NoGil unlocked;
+      Tensor ws;
+      out = empty({Tq, heads, 128}, at::kBFloat16, *q);
+      lse = empty({Tq, heads}, at::kFloat, *q);
+      const int64_t bytes = litedsa_mla_prefill_workspace((int)Tq, (int)Tk, (int)heads);
+      if (bytes > 0) ws = empty({bytes}, at::kByte, *q);
+      rc = litedsa_mla_prefill(q->data_ptr(), q->stride(0), q->stride(1), kn->data_ptr(), kn->stride(0), kn->stride(1), kr->data_ptr(), kr->stride(0),
+                               v->data_ptr(), v->stride(0), v->stride(1), ints(cq), ints(ck), (int)B, (float)sm, a[7] == Py_True, out.data_ptr(),
+                               static_cast<float*>(lse.data_ptr()), (int)Tq, (int)Tk, (int)heads, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                               stream_of(dev));
+    }
+    return rc == LITEDSA_OK ? pair(out, lse) : PyLong_FromLong(rc);
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"sparse_prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sparse_prefill)), METH_FASTCALL, nullptr},
     {"dsv4_c128a_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(dsv4_c128a_bf16)), METH_FASTCALL, nullptr},
     {"dsv4_masked_mla_bf16_out", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(dsv4_masked_mla_bf16_out)), METH_FASTCALL, nullptr},
     {"lite_topk", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(lite_topk)), METH_FASTCALL, nullptr},
+    {"append_kv", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append_kv)), METH_FASTCALL, nullptr},
+    {"mla_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(mla_decode)), METH_FASTCALL, nullptr},
+    {"mla_prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(mla_prefill)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "litedsa_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -62,6 +62,12 @@ def append_kv(kv_c: torch.Tensor, k_rope: torch.Tensor, positions: torch.Tensor,
     Tokens with a slot that is negative or beyond the cache are padding: no row is written for them.  No two tokens may have the same
     slot.  Tokens whose position is not in ``cos_sin`` are left out altogether.
     """
+    if (host := _lib.host()) is not None:
+        r = host.append_kv(kv_c, k_rope, positions, cos_sin, slots, kv_cache, interleaved, q_rope, q_out, k_out)
+        if r is not None:
+            if r is not True:
+                check(r, "append_kv")
+            return
     _need(kv_c, "kv_c", torch.bfloat16, 2)
     _need(k_rope, "k_rope", torch.bfloat16, 2)
     _need(positions, "positions", _INDEX, 1)
@@ -109,6 +115,12 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tenso
     Returns ``(out [B, (q_len,) heads, 512] bf16, lse [B, (q_len,) heads] f32)``, written into ``out`` / ``lse`` when given
     (contiguous).  A row that sees no key: out = 0, lse = +inf.  Lengths are clamped to what a row of the table can hold.
     """
+    if out is None and lse is None and (host := _lib.host()) is not None:
+        r = host.mla_decode(q, kv_cache, block_table, seq_lens, sm_scale)
+        if r is not None:
+            if type(r) is int:
+                check(r, "mla_decode")
+            return r
     _need(q, "q", torch.bfloat16)
     _need(block_table, "block_table", torch.int32, 2)
     _need(seq_lens, "seq_lens", torch.int32, 1)
@@ -165,6 +177,12 @@ def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: 
     Returns ``(out [Tq, heads, 128] bf16, lse [Tq, heads] f32)``, written into ``out`` / ``lse`` when given (contiguous).  A row that sees
     no key: out = 0, lse = +inf.  Rows that are no sequence's (behind ``cu_seqlens_q[-1]``) are not written.
     """
+    if out is None and lse is None and (host := _lib.host()) is not None:
+        r = host.mla_prefill(q, k_nope, k_rope, v, sm_scale, cu_seqlens_q, cu_seqlens_k, causal)
+        if r is not None:
+            if type(r) is int:
+                check(r, "mla_prefill")
+            return r
     for t, n, d in ((q, "q", 3), (k_nope, "k_nope", 3), (k_rope, "k_rope", 2), (v, "v", 3)):
         _need(t, n, torch.bfloat16, d)
         if t.stride(-1) != 1:
