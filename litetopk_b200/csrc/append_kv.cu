@@ -6,9 +6,9 @@
 //   packed    512 e4m3 codes | 4 fp32 scales | 64 bf16: scale = the smallest power of two that brings a group's 128 dims into
 //             +-448, so that code x scale is exact in bf16 and attention over the row rounds nothing again
 //
-// Element-wise and bound by memory; a few tokens by latency, so a token is a block of its own: eight warps of it rotate heads
-// (four lanes a head, eight heads a warp), the last one has the cache row, sixteen latent dims a lane, so that a group's
-// maximum is three shuffles.  Rows are read and written once, 16 bytes an access.
+// Element-wise and bound by memory; a few tokens by latency, so a token is a block of its own: up to eight warps of it rotate heads
+// (eight lanes a head, eight heads a warp), the last one has the cache row, sixteen latent dims a lane, so that a group's
+// maximum is three shuffles.  Everything is read and written once, 16 bytes an access, neighbouring lanes neighbouring bytes.
 #include "common.cuh"
 
 namespace lt {
@@ -25,7 +25,7 @@ struct Params {
   long long kv_c_pitch, k_rope_pitch, cs_pitch, q_in_token, q_in_head, q_out_token, q_out_head, k_out_pitch, block_pitch;
   long long n_rows, n_pos;
   int block_size, heads;
-  int pos64, slot64, packed, interleaved;
+  int pos64, slot64;
 };
 
 __device__ __forceinline__ long long index_at(const void* p, int wide, int i) {
@@ -39,90 +39,91 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// cos and sin of a lane's pairs 8 j .. 8 j + 7
-struct Angles {
-  float c[8], s[8];
+// A vector of 64 dims has eight lanes, 16 bytes each: four pairs of neighbours, or eight dims whose partners lane j ^ 4 has.
+template <bool kInterleaved>
+struct Turn {
+  static constexpr int kPairs = kInterleaved ? 4 : 8;
+  float c[kPairs], s[kPairs];
   __device__ __forceinline__ void load(const float* row, int j) {
+    const int first = kInterleaved ? 4 * j : 8 * (j & 3);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 a = *reinterpret_cast<const float4*>(row + 8 * j + 4 * i), b = *reinterpret_cast<const float4*>(row + 32 + 8 * j + 4 * i);
-      c[4 * i] = a.x; c[4 * i + 1] = a.y; c[4 * i + 2] = a.z; c[4 * i + 3] = a.w;
-      s[4 * i] = b.x; s[4 * i + 1] = b.y; s[4 * i + 2] = b.z; s[4 * i + 3] = b.w;
+    for (int i = 0; i < kPairs; i += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(row + first + i), b = *reinterpret_cast<const float4*>(row + 32 + first + i);
+      c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+      s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
     }
+    if (!kInterleaved && j < 4)                        // x c - y s of the first half, y c + x s of the second
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) s[i] = -s[i];
   }
-};
-// byte offsets of the two 16-byte halves that hold pairs 8 j .. 8 j + 7
-__device__ __forceinline__ int half_at(int interleaved, int j, int half) { return interleaved ? 32 * j + 16 * half : 16 * j + 64 * half; }
-
-__device__ __forceinline__ void rotate(uint4& a, uint4& b, const Angles& t, int interleaved) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(&a);
-  uint32_t* v = reinterpret_cast<uint32_t*>(&b);
-  if (interleaved) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t& w = i < 4 ? u[i] : v[i - 4];
-      const float x = lo_of(w), y = hi_of(w);
-      w = bf16x2(x * t.c[i] - y * t.s[i], y * t.c[i] + x * t.s[i]);
-    }
-  } else {
+  // all 32 lanes
+  __device__ __forceinline__ uint4 operator()(const uint4& v) const {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float x0 = lo_of(u[i]), x1 = hi_of(u[i]), y0 = lo_of(v[i]), y1 = hi_of(v[i]);
-      const int p = 2 * i;
-      u[i] = bf16x2(x0 * t.c[p] - y0 * t.s[p], x1 * t.c[p + 1] - y1 * t.s[p + 1]);
-      v[i] = bf16x2(y0 * t.c[p] + x0 * t.s[p], y1 * t.c[p + 1] + x1 * t.s[p + 1]);
+      const float x = lo_of(u[i]), y = hi_of(u[i]);
+      if (kInterleaved) {
+        o[i] = bf16x2(x * c[i] - y * s[i], y * c[i] + x * s[i]);
+      } else {
+        const uint32_t w = __shfl_xor_sync(0xffffffffu, u[i], 4);
+        o[i] = bf16x2(x * c[(2 * i) % kPairs] + lo_of(w) * s[(2 * i) % kPairs], y * c[(2 * i + 1) % kPairs] + hi_of(w) * s[(2 * i + 1) % kPairs]);
+      }
     }
+    return make_uint4(o[0], o[1], o[2], o[3]);
   }
-}
+};
 
+template <bool kInterleaved, bool kPacked>
 __global__ void __launch_bounds__(32 * (kMaxHeadWarps + 1)) append_kv_kernel(const Params p) {
   const int t = (int)blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head_warps = (blockDim.x >> 5) - 1;
-  const int j = lane & 3;
+  const int j = lane & 7;
   pdl_trigger();
   pdl_wait();
   const long long pos = index_at(p.positions, p.pos64, t);
-  if (pos < 0 || pos >= p.n_pos) return;               // not in the table: the token is left out
-  const float* cs = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.cos_sin) + pos * p.cs_pitch);
+  const bool known = pos >= 0 && pos < p.n_pos;        // not in the table: the token is left out
+  const float* angles = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.cos_sin) + pos * p.cs_pitch);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  Turn<kInterleaved> turn;
   if (warp < head_warps) {
-    Angles ang;
-    ang.load(cs, j);
-    for (int h = 8 * warp + (lane >> 2); h < p.heads; h += 8 * head_warps) {
-      const uint8_t* src = p.q_in + t * p.q_in_token + h * p.q_in_head;
-      uint8_t* dst = p.q_out + t * p.q_out_token + h * p.q_out_head;
-      uint4 a = load16(src + half_at(p.interleaved, j, 0)), b = load16(src + half_at(p.interleaved, j, 1));
-      rotate(a, b, ang, p.interleaved);
-      *reinterpret_cast<uint4*>(dst + half_at(p.interleaved, j, 0)) = a;
-      *reinterpret_cast<uint4*>(dst + half_at(p.interleaved, j, 1)) = b;
+    // (the first heads are on their way while the position and its angles are looked up)
+    const uint8_t* src = p.q_in + t * p.q_in_token + 16 * j;
+    uint8_t* dst = p.q_out + t * p.q_out_token + 16 * j;
+    int h = 8 * warp + (lane >> 3);
+    uint4 a = h < p.heads ? load16(src + h * p.q_in_head) : zero, b = h + 4 < p.heads ? load16(src + (h + 4) * p.q_in_head) : zero;
+    if (!known) return;
+    turn.load(angles, j);
+    for (;;) {
+      a = turn(a);
+      b = turn(b);
+      if (h < p.heads) *reinterpret_cast<uint4*>(dst + h * p.q_out_head) = a;
+      if (h + 4 < p.heads) *reinterpret_cast<uint4*>(dst + (h + 4) * p.q_out_head) = b;
+      h += 8 * head_warps;
+      if (h - (lane >> 3) >= p.heads) return;
+      a = h < p.heads ? load16(src + h * p.q_in_head) : zero;
+      b = h + 4 < p.heads ? load16(src + (h + 4) * p.q_in_head) : zero;
     }
-    return;
   }
+  if (!known) return;
+  turn.load(angles, j);
   const long long slot = index_at(p.slots, p.slot64, t);
   uint8_t* row = nullptr;
   if (slot >= 0 && slot < p.n_rows)
-    row = p.cache + (slot / p.block_size) * p.block_pitch + (slot % p.block_size) * (p.packed ? 656 : 1152);
-  if (lane < 4) {
-    Angles ang;
-    ang.load(cs, j);
-    const uint8_t* src = p.k_rope + t * p.k_rope_pitch;
-    uint4 a = load16(src + half_at(p.interleaved, j, 0)), b = load16(src + half_at(p.interleaved, j, 1));
-    rotate(a, b, ang, p.interleaved);
-    uint8_t* dst[2] = {row ? row + (p.packed ? 528 : 1024) : nullptr, p.k_out ? p.k_out + t * p.k_out_pitch : nullptr};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (dst[i]) {
-        *reinterpret_cast<uint4*>(dst[i] + half_at(p.interleaved, j, 0)) = a;
-        *reinterpret_cast<uint4*>(dst[i] + half_at(p.interleaved, j, 1)) = b;
-      }
+    row = p.cache + (slot / p.block_size) * p.block_pitch + (slot % p.block_size) * (kPacked ? 656 : 1152);
+  const uint4 k = turn(lane < 8 ? load16(p.k_rope + t * p.k_rope_pitch + 16 * j) : zero);
+  if (lane < 8) {
+    if (row) *reinterpret_cast<uint4*>(row + (kPacked ? 528 : 1024) + 16 * j) = k;
+    if (p.k_out) *reinterpret_cast<uint4*>(p.k_out + t * p.k_out_pitch + 16 * j) = k;
   }
   if (!row) return;                                    // padding, or no row of this cache (warp-uniform)
-  __syncwarp();
-  const uint8_t* src = p.kv_c + t * p.kv_c_pitch + 32 * lane;
-  const uint4 a = load16(src), b = load16(src + 16);
-  if (!p.packed) {
-    *reinterpret_cast<uint4*>(row + 32 * lane) = a;
-    *reinterpret_cast<uint4*>(row + 32 * lane + 16) = b;
+  const uint8_t* src = p.kv_c + t * p.kv_c_pitch;
+  if (!kPacked) {
+    const uint4 a = load16(src + 16 * lane), b = load16(src + 512 + 16 * lane);
+    *reinterpret_cast<uint4*>(row + 16 * lane) = a;
+    *reinterpret_cast<uint4*>(row + 512 + 16 * lane) = b;
     return;
   }
+  const uint4 a = load16(src + 32 * lane), b = load16(src + 32 * lane + 16);
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   uint32_t amax = 0;                                   // of the magnitudes' bits: bf16 in the upper half of a float
 #pragma unroll
@@ -177,7 +178,12 @@ extern "C" int litedsa_append_kv(const void* kv_c, int64_t kv_c_stride, const vo
   p.k_out_pitch = 2 * k_out_stride; p.block_pitch = block_stride_bytes;
   p.n_rows = n_blocks * block_size; p.n_pos = n_positions;
   p.block_size = block_size; p.heads = q_rope ? heads : 0;
-  p.pos64 = positions_64; p.slot64 = slots_64; p.packed = packed; p.interleaved = interleaved;
+  p.pos64 = positions_64; p.slot64 = slots_64;
   const int warps = min(append::kMaxHeadWarps, (p.heads + 7) / 8) + 1;
-  return launch_pdl(append::append_kv_kernel, dim3((unsigned)T), 32 * warps, 0, reinterpret_cast<cudaStream_t>(stream), p);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)T);
+  if (interleaved) return packed ? launch_pdl(append::append_kv_kernel<true, true>, grid, 32 * warps, 0, st, p)
+                                 : launch_pdl(append::append_kv_kernel<true, false>, grid, 32 * warps, 0, st, p);
+  return packed ? launch_pdl(append::append_kv_kernel<false, true>, grid, 32 * warps, 0, st, p)
+                : launch_pdl(append::append_kv_kernel<false, false>, grid, 32 * warps, 0, st, p);
 }
