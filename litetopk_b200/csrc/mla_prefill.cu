@@ -70,6 +70,11 @@ struct Params {
 enum { kSiteFull = 1, kSiteEmpty, kSiteQ, kSiteQFree, kSiteS, kSiteP, kSiteO, kSiteWork, kSiteWorkEmpty, kSiteClc };
 static __device__ int g_status[8];
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -383,8 +388,9 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   } else {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
    if (warp == kWarpMma) {
-    // ------------------------------------------------------------ the products (one thread)
-    if (lane == 0) {
+    // ------------------------------------------------------------ the products (one thread: elected, so that the compiler knows the
+    // descriptors to be the warp's; under a branch on the lane a product took 110 to 130 cycles to issue, of which it computes 64)
+    if (elect_one()) {
       constexpr uint32_t idesc_qk = umma_idesc(1, 1, false, false, 128, 128), idesc_pv = umma_idesc(1, 1, false, true, 128, 128),
                          idesc_half = umma_idesc(1, 1, false, true, 128, 64);
       const uint64_t q_desc = umma_desc(sbase + kOffQ, 16, 1024, kSwz128), k_desc = umma_desc(sbase + kOffRing, 16, 1024, kSwz128),
