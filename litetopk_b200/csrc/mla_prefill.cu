@@ -35,7 +35,10 @@ constexpr int kWarpMma = 8, kWarpLoad = 9, kThreads = 384;     // (warps 10 and 
 constexpr uint32_t kTmemO = 256;                            // S0, S1, O0, O1: 128 columns each
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kMInit = -1e30f;
-constexpr float kOvershoot = 8.f;
+// P is relative to a maximum that may be stale: a block's exponentials are computed with the row's last one, and only if their sum
+// shows that some were above it by more than this is the maximum taken anew, O rescaled and the block repeated.  A pass over the scores for
+// their maximum cost a quarter of a row's softmax; P is as exact in bf16 above one as below, and fp32 sums hold 2^32 as well as 1.
+constexpr float kMostSum = 4294967296.f;
 
 struct Work {
   int head, q0, rows;          // queries [q0, q0 + rows) of the call's tokens
@@ -265,57 +268,77 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ok = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[t], ns & 1, wt, kSiteS, i));
         if (!ok) break;
         tc_fence_after();
-        float s[128];
+        const int key0 = (k.b0 + i) * kBlock, seen = lim - key0;
+        const bool masked = key0 + kBlock > low;
+        uint32_t w[64];
+        uint64_t sum[4];
+        for (bool anew = i == 0;;) {
+          float v[2][32];
+          tmem_ld32(s_col, v[0]);
+          if (anew) {
+            float top = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld32(s_col + 32 * x, s + 32 * x);
-        tmem_wait_ld();
-        const int key0 = (k.b0 + i) * kBlock;
-        if (key0 + kBlock > low) {
-          const int seen = lim - key0;
+            for (int x = 0; x < 4; ++x) {
+              float (&a)[32] = v[x & 1];
+              tmem_wait_ld();
+              if (x < 3) tmem_ld32(s_col + 32 * (x + 1), v[(x + 1) & 1]);
+              if (masked)
 #pragma unroll
-          for (int x = 0; x < 128; ++x) s[x] = x < seen ? s[x] : -INFINITY;
-        }
-        float mx[4];
+                for (int y = 0; y < 32; ++y) a[y] = 32 * x + y < seen ? a[y] : -INFINITY;
+              float mx[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) mx[x] = fmaxf(s[x], s[x + 4]);
+              for (int y = 0; y < 4; ++y) mx[y] = fmaxf(a[y], a[y + 4]);
 #pragma unroll
-        for (int x = 8; x < 128; x += 8)
+              for (int y = 8; y < 32; y += 8)
 #pragma unroll
-          for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], fmaxf(s[x + y], s[x + y + 4]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (i == 0) {
-          m = fmaxf(m, top);
-        } else if (__any_sync(0xffffffffu, (top - m) * c > kOvershoot)) {      // (the S that is here is behind the PV before it)
-          const float now = fmaxf(m, top), f = fast_exp2((m - now) * c);
-          m = now;
-          l *= f;
+                for (int z = 0; z < 4; ++z) mx[z] = fmaxf(mx[z], fmaxf(a[y + z], a[y + z + 4]));
+              top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            }
+            tmem_ld32(s_col, v[0]);
+            const float now = fmaxf(m, top), f = fast_exp2((m - now) * c);
+            m = now;
+            if (i > 0) {                                                    // (the S that is here is behind the PV before it)
+              l *= f;
 #pragma unroll 1
-          for (int x = 0; x < 128; x += 32) {
-            float o[32];
-            tmem_ld32(o_col + x, o);
+              for (int x = 0; x < 128; x += 32) {
+                float o[32];
+                tmem_ld32(o_col + x, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= f;
+                tmem_st32(o_col + x, o);
+              }
+            }
+          }
+          const float mc = -m * c;
+          const uint64_t m2 = pack2(mc, mc);
+          sum[0] = sum[1] = sum[2] = sum[3] = 0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float (&a)[32] = v[x & 1];
             tmem_wait_ld();
+            if (x < 3) tmem_ld32(s_col + 32 * (x + 1), v[(x + 1) & 1]);
+            if (masked)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_st32(o_col + x, o);
+              for (int y = 0; y < 32; ++y) a[y] = 32 * x + y < seen ? a[y] : -INFINITY;
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              const float2 e = unpack2(fma2(pack2(a[2 * y], a[2 * y + 1]), c2, m2));
+              const float b0 = fast_exp2(e.x), b1 = fast_exp2(e.y);
+              sum[y & 3] = add2(sum[y & 3], pack2(b0, b1));
+              w[16 * x + y] = bf16x2(b0, b1);
+            }
           }
-        }
-        const float mc = -m * c;
-        const uint64_t m2 = pack2(mc, mc);
-        uint64_t sum[2] = {0, 0};
-#pragma unroll
-        for (int x = 0; x < 128; x += 32) {
-          uint32_t w[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            const float2 e = unpack2(fma2(pack2(s[x + 2 * y], s[x + 2 * y + 1]), c2, m2));
-            const float a = fast_exp2(e.x), b = fast_exp2(e.y);
-            sum[y & 1] = add2(sum[y & 1], pack2(a, b));
-            w[y] = bf16x2(a, b);
+          sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+          const float2 both = unpack2(sum[0]);
+          if (anew || !__any_sync(0xffffffffu, !(both.x + both.y <= kMostSum))) {
+            l += both.x + both.y;
+            break;
           }
-          tmem_st16(s_col + x / 2, w);
+          anew = true;
         }
-        const float2 both = unpack2(add2(sum[0], sum[1]));
-        l += both.x + both.y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_st16(s_col + 16 * x, w + 16 * x);
         tmem_wait_st();
         const int valid = k.nk - key0;
         if (valid < kBlock) {
