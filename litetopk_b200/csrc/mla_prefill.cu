@@ -49,7 +49,8 @@ struct Work {
   int live;                    // 0: no more work
 };
 struct Misc {
-  uint64_t full[kRing], empty[kRing], q_full[2], q_free[2], s_ready[2], p_ready[2], o_done[2], work_full[2], work_empty[2], clc, drained;
+  uint64_t k_full[2], v_full[2], k_free[2], v_free[2];      // by the parity of the block
+  uint64_t q_full[2], q_free[2], s_ready[2], p_ready[2][2], half_done[2], o_done[2], work_full[2], work_empty[2], clc, drained;
   uint4 clc_answer;
   Work work[2];
   uint32_t left, tmem_base;
@@ -209,9 +210,10 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRing; ++i) { mbar_init(&ms.full[i], 1); mbar_init(&ms.empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ms.q_full[i], 1); mbar_init(&ms.q_free[i], 1); mbar_init(&ms.s_ready[i], 1); mbar_init(&ms.p_ready[i], 4);
+      mbar_init(&ms.k_full[i], 1); mbar_init(&ms.v_full[i], 1); mbar_init(&ms.k_free[i], 1); mbar_init(&ms.v_free[i], 1);
+      mbar_init(&ms.q_full[i], 1); mbar_init(&ms.q_free[i], 1); mbar_init(&ms.s_ready[i], 1);
+      mbar_init(&ms.p_ready[i][0], 4); mbar_init(&ms.p_ready[i][1], 4); mbar_init(&ms.half_done[i], 1);
       mbar_init(&ms.o_done[i], 1); mbar_init(&ms.work_full[i], 1); mbar_init(&ms.work_empty[i], 9);
     }
     mbar_init(&ms.clc, 1);
@@ -268,96 +270,86 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ok = __all_sync(0xffffffffu, mbar_wait(&ms.s_ready[t], ns & 1, wt, kSiteS, i));
         if (!ok) break;
         tc_fence_after();
-        const int key0 = (k.b0 + i) * kBlock, seen = lim - key0;
-        const bool masked = key0 + kBlock > low;
-        uint32_t w[64];
-        uint64_t sum[4];
-        for (bool anew = i == 0;;) {
-          float v[2][32];
-          tmem_ld32(s_col, v[0]);
-          if (anew) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float (&a)[32] = v[x & 1];
-              tmem_wait_ld();
-              if (x < 3) tmem_ld32(s_col + 32 * (x + 1), v[(x + 1) & 1]);
-              if (masked)
-#pragma unroll
-                for (int y = 0; y < 32; ++y) a[y] = 32 * x + y < seen ? a[y] : -INFINITY;
-              float mx[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y) mx[y] = fmaxf(a[y], a[y + 4]);
-#pragma unroll
-              for (int y = 8; y < 32; y += 8)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) mx[z] = fmaxf(mx[z], fmaxf(a[y + z], a[y + z + 4]));
-              top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-            }
-            tmem_ld32(s_col, v[0]);
-            const float now = fmaxf(m, top), f = fast_exp2((m - now) * c);
-            m = now;
-            if (i > 0) {                                                    // (the S that is here is behind the PV before it)
-              l *= f;
-#pragma unroll 1
-              for (int x = 0; x < 128; x += 32) {
-                float o[32];
-                tmem_ld32(o_col + x, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= f;
-                tmem_st32(o_col + x, o);
-              }
-            }
-          }
-          const float mc = -m * c;
-          const uint64_t m2 = pack2(mc, mc);
-          sum[0] = sum[1] = sum[2] = sum[3] = 0;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float (&a)[32] = v[x & 1];
-            tmem_wait_ld();
-            if (x < 3) tmem_ld32(s_col + 32 * (x + 1), v[(x + 1) & 1]);
-            if (masked)
-#pragma unroll
-              for (int y = 0; y < 32; ++y) a[y] = 32 * x + y < seen ? a[y] : -INFINITY;
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              const float2 e = unpack2(fma2(pack2(a[2 * y], a[2 * y + 1]), c2, m2));
-              const float b0 = fast_exp2(e.x), b1 = fast_exp2(e.y);
-              sum[y & 3] = add2(sum[y & 3], pack2(b0, b1));
-              w[16 * x + y] = bf16x2(b0, b1);
-            }
-          }
-          sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-          const float2 both = unpack2(sum[0]);
-          if (anew || !__any_sync(0xffffffffu, !(both.x + both.y <= kMostSum))) {
-            l += both.x + both.y;
-            break;
-          }
-          anew = true;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_st16(s_col + 16 * x, w + 16 * x);
-        tmem_wait_st();
+        const int key0 = (k.b0 + i) * kBlock;
         const int valid = k.nk - key0;
         if (valid < kBlock) {
           // Value rows behind the sequence's end: zeros, whatever lies there.  (Both tiles write them; the block's other granules are
           // in nobody's way, and the slots are not given back before this tile's PV.)
-          const int from = max(valid, 0);
+          const int from = max(valid, 0), b = block0 + i;
+          ok = __all_sync(0xffffffffu, mbar_wait(&ms.v_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i)) && ok;
 #pragma unroll 1
           for (int j = 3; j < kPerBlock; ++j) {
-            const int g = kPerBlock * (block0 + i) + j;
-            ok = __all_sync(0xffffffffu, mbar_wait(&ms.full[g & 7], (g >> 3) & 1, wt, kSiteFull, i)) && ok;
+            const int g = kPerBlock * b + j;
             const uint32_t base = sbase + kOffRing + (uint32_t)(g & 7) * kGranule;
             for (int x = r; x < (kBlock - from) * 8; x += kRows)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + from * 128 + 16 * x), "r"(0) : "memory");
           }
           fence_proxy_async_smem();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ms.p_ready[t]);
+        // The block's two halves one after the other: the first one's product runs while the second is computed.
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int seen = lim - key0 - 64 * h;
+          const bool masked = key0 + 64 * (h + 1) > low;
+          uint32_t w[32];
+          for (bool anew = i + h == 0;;) {
+            float v[2][32];
+            tmem_ld32(s_col + 64 * h, v[0]);
+            tmem_ld32(s_col + 64 * h + 32, v[1]);
+            tmem_wait_ld();
+            if (masked)
+#pragma unroll
+              for (int x = 0; x < 64; ++x) v[x >> 5][x & 31] = x < seen ? v[x >> 5][x & 31] : -INFINITY;
+            if (anew) {
+              float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int x = 0; x < 64; x += 8)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) mx[z] = fmaxf(mx[z], fmaxf(v[x >> 5][(x & 31) + z], v[x >> 5][(x & 31) + z + 4]));
+              const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))), f = fast_exp2((m - now) * c);
+              m = now;
+              l *= f;
+              if (i + h > 0) {
+                // (the PV of the block before is complete where S is there; that of this one's first half, if this is the second, has been issued)
+                if (h > 0) {
+                  ok = __all_sync(0xffffffffu, mbar_wait(&ms.half_done[t], ns & 1, wt, kSiteP, i)) && ok;
+                  tc_fence_after();
+                }
+#pragma unroll 1
+                for (int x = 0; x < 128; x += 32) {
+                  float o[32];
+                  tmem_ld32(o_col + x, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) o[e] *= f;
+                  tmem_st32(o_col + x, o);
+                }
+              }
+            }
+            const float mc = -m * c;
+            const uint64_t m2 = pack2(mc, mc);
+            uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int y = 0; y < 32; ++y) {
+              const float2 e = unpack2(fma2(pack2(v[y >> 4][2 * (y & 15)], v[y >> 4][2 * (y & 15) + 1]), c2, m2));
+              const float2 r = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+              sum[y & 3] = add2(sum[y & 3], pack2(r.x, r.y));
+              w[y] = bf16x2(r.x, r.y);
+            }
+            const float2 both = unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+            if (anew || !__any_sync(0xffffffffu, !(both.x + both.y <= kMostSum))) {
+              l += both.x + both.y;
+              break;
+            }
+            anew = true;
+          }
+          tmem_st16(s_col + 32 * h, w);
+          tmem_st16(s_col + 32 * h + 16, w + 16);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ms.p_ready[t][h]);
+        }
       }
       if (!ok) break;
       block0 += max(k.n[0], k.n[1]);
@@ -428,40 +420,44 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (!live) break;
         auto count = [&](int t) { return t ? n1 : n0; };
         auto last_user = [&](int t, int i) { return t == (i < n1 ? 1 : 0); };
+        auto first_user = [&](int t, int i) { return t == (i < n0 ? 0 : 1); };
         auto qk = [&](int t, int i) {
-          for (int j = 0; j < 3; ++j) {
-            const int g = kPerBlock * (block0 + i) + j;
-            if (!(ok = mbar_wait(&ms.full[g & 7], (g >> 3) & 1, wt, kSiteFull, i))) return;
-            tc_fence_after();
+          const int b = block0 + i;
+          if (first_user(t, i) && !(ok = mbar_wait(&ms.k_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i))) return;
+          tc_fence_after();
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              mma_ss(tmem + 128 * t, q_desc + ((kQTile * t + kGranule * j) >> 4) + 2 * x, k_desc + (uint32_t)(g & 7) * (kGranule >> 4) + 2 * x, idesc_qk,
-                     (uint32_t)(j | x));
-            if (last_user(t, i)) mma_commit_cta(&ms.empty[g & 7]);
+          for (int j = 0; j < 3; ++j) {
+            const uint64_t kd = k_desc + (uint32_t)((kPerBlock * b + j) & 7) * (kGranule >> 4), qd = q_desc + ((kQTile * t + kGranule * j) >> 4);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) mma_ss(tmem + 128 * t, qd + 2 * x, kd + 2 * x, idesc_qk, (uint32_t)(j | x));
           }
           mma_commit_cta(&ms.s_ready[t]);
+          if (last_user(t, i)) mma_commit_cta(&ms.k_free[b & 1]);
           if (i + 1 == count(t)) mma_commit_cta(&ms.q_free[t]);
         };
         auto pv = [&](int t, int i) {
-          if (!(ok = mbar_wait(&ms.p_ready[t], np[t] & 1, wt, kSiteP, i))) return;
-          ++np[t];
-          const int g = kPerBlock * (block0 + i) + 3;
-          for (int j = 0; j < 2; ++j)
-            if (!(ok = mbar_wait(&ms.full[(g + j) & 7], ((g + j) >> 3) & 1, wt, kSiteFull, i))) return;
-          tc_fence_after();
+          const int b = block0 + i, g = kPerBlock * b + 3;
+          if (first_user(t, i) && !(ok = mbar_wait(&ms.v_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i))) return;
           const uint32_t d = tmem + kTmemO + 128 * t, a = tmem + 128 * t;
           const uint64_t v0 = v_desc + (uint32_t)(g & 7) * (kGranule >> 4);
-          if ((g & 7) != 7) {
+          const bool split = (g & 7) == 7;                    // the block's two granules of V lie at the ring's two ends
 #pragma unroll
-            for (int x = 0; x < 8; ++x) mma_ts(d, a + 8 * x, v0 + 128 * x, idesc_pv, (uint32_t)(i | x));
-          } else {                                            // the block's two granules of V lie at the ring's two ends
+          for (int h = 0; h < 2; ++h) {
+            if (!(ok = mbar_wait(&ms.p_ready[t][h], np[t] & 1, wt, kSiteP, i))) return;
+            tc_fence_after();
+            if (!split) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+              for (int x = 4 * h; x < 4 * h + 4; ++x) mma_ts(d, a + 8 * x, v0 + 128 * x, idesc_pv, (uint32_t)(i | x));
+            } else {
 #pragma unroll
-              for (int x = 0; x < 8; ++x) mma_ts(d + 64 * j, a + 8 * x, (j ? v_desc : v0) + 128 * x, idesc_half, (uint32_t)(i | x));
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int x = 4 * h; x < 4 * h + 4; ++x) mma_ts(d + 64 * j, a + 8 * x, (j ? v_desc : v0) + 128 * x, idesc_half, (uint32_t)(i | x));
+            }
+            if (h == 0) mma_commit_cta(&ms.half_done[t]);
           }
-          if (last_user(t, i))
-            for (int j = 0; j < 2; ++j) mma_commit_cta(&ms.empty[(g + j) & 7]);
+          ++np[t];
+          if (last_user(t, i)) mma_commit_cta(&ms.v_free[b & 1]);
           if (i + 1 == count(t)) mma_commit_cta(&ms.o_done[t]);
         };
         for (int t = 0; t < 2 && ok; ++t)
@@ -490,7 +486,7 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint64_t once = l2_policy_evict_first();
     uint64_t keep;
     asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(keep));
-    int w = (int)blockIdx.x, block0 = 0, asked = 0, nq[2] = {0, 0}, clc_asked = 0, clc_got = 0;
+    int w = (int)blockIdx.x, block0 = 0, asked[2] = {0, 0}, nq[2] = {0, 0}, clc_asked = 0, clc_got = 0;
     bool ok = true;
     for (int it = 0; ok;) {
       if (w == 0 && lane == 0 && p.plan) *p.plan = make_int4(tiles, cut.whole, cut.pieces, 0);
@@ -525,16 +521,23 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           const int n = max(k.n[0], k.n[1]);
           for (int i = 0; i < n && ok; ++i) {
             const int at = k.k0 + (k.b0 + i) * kBlock;
+            // Granule g takes the place of g - 8: of K's last of two blocks before, V's two, and K's first two of the block before.
+            const int b = block0 + i;
             for (int j = 0; j < kPerBlock; ++j) {
-              const int g = kPerBlock * (block0 + i) + j;
-              uint64_t* bar = &ms.full[g & 7];
-              const uint32_t dst = sbase + kOffRing + (uint32_t)(g & 7) * kGranule;
-              if (g >= kRing && !(ok = mbar_wait(&ms.empty[g & 7], ((g >> 3) & 1) ^ 1, wt, kSiteEmpty, i))) break;
-              mbar_arrive_expect_tx(bar, kGranule);
+              uint64_t* bar = j < 3 ? &ms.k_full[b & 1] : &ms.v_full[b & 1];
+              const uint32_t dst = sbase + kOffRing + (uint32_t)((kPerBlock * b + j) & 7) * kGranule;
+              const int old = j < 3 ? b - 2 : b - 1;
+              if (old >= 0 && j != 2 && j != 4) {
+                uint64_t* freed = j == 1 ? &ms.v_free[old & 1] : &ms.k_free[old & 1];
+                if (!(ok = mbar_wait(freed, (old >> 1) & 1, wt, kSiteEmpty, i))) break;
+              }
+              if (j == 0 || j == 3) {
+                mbar_arrive_expect_tx(bar, (j == 0 ? 3 : 2) * kGranule);
+                ++asked[j == 3];
+              }
               if (j < 2) tma_load_3d_hint(dst, &map_kn, 64 * j, k.head, at, bar, keep);
               else if (j == 2) tma_load_2d_hint(dst, &map_kr, 0, at, bar, keep);
               else tma_load_3d_hint(dst, &map_v, 64 * (j - 3), k.head, at, bar, keep);
-              asked = g + 1;
             }
           }
           block0 += n;
@@ -553,7 +556,9 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       w = __shfl_sync(0xffffffffu, next, 0);
     }
     if (!ok && lane == 0) {                                   // given up: what is in flight lands first
-      for (int g = max(asked - kRing, 0); g < asked; ++g) mbar_drain(&ms.full[g & 7], (g >> 3) & 1);
+      // (K's last granules may not have been requested: then the barrier's phase does not end, and the limit does)
+      for (int b = max(asked[0] - 2, 0); b < asked[0]; ++b) mbar_drain(&ms.k_full[b & 1], (b >> 1) & 1);
+      for (int b = max(asked[1] - 2, 0); b < asked[1]; ++b) mbar_drain(&ms.v_full[b & 1], (b >> 1) & 1);
       for (int t = 0; t < 2; ++t)
         if (nq[t] > 0) mbar_drain(&ms.q_full[t], (nq[t] - 1) & 1);
       if (clc_asked > clc_got) mbar_drain(&ms.clc, clc_got & 1);
