@@ -410,69 +410,81 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                          idesc_half = umma_idesc(1, 1, false, true, 128, 64);
       const uint64_t q_desc = umma_desc(sbase + kOffQ, 16, 1024, kSwz128), k_desc = umma_desc(sbase + kOffRing, 16, 1024, kSwz128),
                      v_desc = umma_desc(sbase + kOffRing, kGranule, 1024, kSwz128);
-      int block0 = 0, nq[2] = {0, 0}, np[2] = {0, 0};
-      bool ok = true;
+      // A tile's second product of a block is issued in front of its next first one, of the next work if there is no more in this: while
+      // the tile with the longer reach finishes a work, the other begins the next.
+      struct Due { int b, first, last, wait_v, free_v; };     // block, whether O begins and ends with it, whether V is first or last used
+      Due due[2];
+      int nq[2] = {0, 0}, np[2] = {0, 0}, block0 = 0;
+      bool has[2] = {false, false}, ok = true;
+      auto pv = [&](int t) {
+        if (!has[t]) return;
+        has[t] = false;
+        const Due& x = due[t];
+        const int b = x.b, g = kPerBlock * b + 3;
+        if (x.wait_v && !(ok = mbar_wait(&ms.v_full[b & 1], (b >> 1) & 1, wt, kSiteFull, b))) return;
+        const uint32_t d = tmem + kTmemO + 128 * t, a = tmem + 128 * t;
+        const uint64_t v0 = v_desc + (uint32_t)(g & 7) * (kGranule >> 4);
+        const bool split = (g & 7) == 7;                      // the block's two granules of V lie at the ring's two ends
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!(ok = mbar_wait(&ms.p_ready[t][h], np[t] & 1, wt, kSiteP, b))) return;
+          tc_fence_after();
+          if (!split) {
+#pragma unroll
+            for (int y = 4 * h; y < 4 * h + 4; ++y) mma_ts(d, a + 8 * y, v0 + 128 * y, idesc_pv, y == 0 && x.first ? 0u : 1u);
+          } else {
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+              for (int y = 4 * h; y < 4 * h + 4; ++y) mma_ts(d + 64 * z, a + 8 * y, (z ? v_desc : v0) + 128 * y, idesc_half, y == 0 && x.first ? 0u : 1u);
+          }
+          if (h == 0) mma_commit_cta(&ms.half_done[t]);
+        }
+        ++np[t];
+        if (x.free_v) mma_commit_cta(&ms.v_free[b & 1]);
+        if (x.last) mma_commit_cta(&ms.o_done[t]);
+      };
       for (int it = 0; ok; ++it) {
-        if (!(ok = mbar_wait(&ms.work_full[it & 1], (it >> 1) & 1, wt, kSiteWork, it))) break;
+        if (!mbar_test(&ms.work_full[it & 1], (it >> 1) & 1)) {            // nothing to go on with yet
+          pv(0);
+          if (ok) pv(1);
+        }
+        if (!ok || !(ok = mbar_wait(&ms.work_full[it & 1], (it >> 1) & 1, wt, kSiteWork, it))) break;
         const Work& k = ms.work[it & 1];
         const int n0 = k.n[0], n1 = k.n[1], live = k.live, n = max(n0, n1);
         mbar_arrive(&ms.work_empty[it & 1]);
         if (!live) break;
-        auto count = [&](int t) { return t ? n1 : n0; };
-        auto last_user = [&](int t, int i) { return t == (i < n1 ? 1 : 0); };
-        auto first_user = [&](int t, int i) { return t == (i < n0 ? 0 : 1); };
-        auto qk = [&](int t, int i) {
-          const int b = block0 + i;
-          if (first_user(t, i) && !(ok = mbar_wait(&ms.k_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i))) return;
-          tc_fence_after();
-#pragma unroll
-          for (int j = 0; j < 3; ++j) {
-            const uint64_t kd = k_desc + (uint32_t)((kPerBlock * b + j) & 7) * (kGranule >> 4), qd = q_desc + ((kQTile * t + kGranule * j) >> 4);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) mma_ss(tmem + 128 * t, qd + 2 * x, kd + 2 * x, idesc_qk, (uint32_t)(j | x));
-          }
-          mma_commit_cta(&ms.s_ready[t]);
-          if (last_user(t, i)) mma_commit_cta(&ms.k_free[b & 1]);
-          if (i + 1 == count(t)) mma_commit_cta(&ms.q_free[t]);
-        };
-        auto pv = [&](int t, int i) {
-          const int b = block0 + i, g = kPerBlock * b + 3;
-          if (first_user(t, i) && !(ok = mbar_wait(&ms.v_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i))) return;
-          const uint32_t d = tmem + kTmemO + 128 * t, a = tmem + 128 * t;
-          const uint64_t v0 = v_desc + (uint32_t)(g & 7) * (kGranule >> 4);
-          const bool split = (g & 7) == 7;                    // the block's two granules of V lie at the ring's two ends
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!(ok = mbar_wait(&ms.p_ready[t][h], np[t] & 1, wt, kSiteP, i))) return;
-            tc_fence_after();
-            if (!split) {
-#pragma unroll
-              for (int x = 4 * h; x < 4 * h + 4; ++x) mma_ts(d, a + 8 * x, v0 + 128 * x, idesc_pv, (uint32_t)(i | x));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int x = 4 * h; x < 4 * h + 4; ++x) mma_ts(d + 64 * j, a + 8 * x, (j ? v_desc : v0) + 128 * x, idesc_half, (uint32_t)(i | x));
-            }
-            if (h == 0) mma_commit_cta(&ms.half_done[t]);
-          }
-          ++np[t];
-          if (last_user(t, i)) mma_commit_cta(&ms.v_free[b & 1]);
-          if (i + 1 == count(t)) mma_commit_cta(&ms.o_done[t]);
-        };
-        for (int t = 0; t < 2 && ok; ++t)
-          if (count(t) > 0) {
-            if ((ok = mbar_wait(&ms.q_full[t], nq[t] & 1, wt, kSiteQ, it))) { ++nq[t]; qk(t, 0); }
-          }
-        // Q_t K(i + 1) writes S over the P that P_t V(i) reads.  Both are issued by this thread, and a CTA's products go through its
+        // Q_t K(i) writes S over the P that P_t V(i - 1) reads.  Both are issued by this thread, and a CTA's products go through its
         // tensor core in the order of issue: the reads of the earlier are behind it when the later's first results are written.
         for (int i = 0; i < n && ok; ++i)
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (i < count(t)) pv(t, i);
-            if (ok && i + 1 < count(t)) qk(t, i + 1);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int mine = t ? n1 : n0, others = t ? n0 : n1, b = block0 + i;
+            if (ok) pv(t);
+            if (!ok || i >= mine) continue;
+            const bool first_user = t == 0 || i >= others, last_user = t == 1 || i >= others;
+            if (i == 0) {
+              if (!(ok = mbar_wait(&ms.q_full[t], nq[t] & 1, wt, kSiteQ, it))) continue;
+              ++nq[t];
+            }
+            if (first_user && !(ok = mbar_wait(&ms.k_full[b & 1], (b >> 1) & 1, wt, kSiteFull, i))) continue;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {
+              const uint64_t kd = k_desc + (uint32_t)((kPerBlock * b + j) & 7) * (kGranule >> 4), qd = q_desc + ((kQTile * t + kGranule * j) >> 4);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) mma_ss(tmem + 128 * t, qd + 2 * x, kd + 2 * x, idesc_qk, (uint32_t)(j | x));
+            }
+            mma_commit_cta(&ms.s_ready[t]);
+            if (last_user) mma_commit_cta(&ms.k_free[b & 1]);
+            if (i + 1 == mine) mma_commit_cta(&ms.q_free[t]);
+            due[t] = Due{b, i == 0, i + 1 == mine, first_user, last_user};
+            has[t] = true;
           }
         block0 += n;
       }
+      if (ok) pv(0);
+      if (ok) pv(1);
       if (!ok) {                                              // given up: what has been issued ends before the tensor memory goes
         mma_commit_cta(&ms.drained);
         mbar_drain(&ms.drained, 0);
@@ -510,14 +522,14 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (!ok || w < 0) break;
         if (lane == 0) {
-          for (int t = 0; t < 2 && ok; ++t)
-            if (k.n[t] > 0) {
-              if (nq[t] > 0 && !(ok = mbar_wait(&ms.q_free[t], (nq[t] - 1) & 1, wt, kSiteQFree, it))) break;
-              mbar_arrive_expect_tx(&ms.q_full[t], kQTile);
-              for (int j = 0; j < 3; ++j)
-                tma_load_3d_hint(sbase + kOffQ + kQTile * t + kGranule * j, &map_q, 64 * j, k.head, k.q0 + kRows * t, &ms.q_full[t], once);
-              ++nq[t];
-            }
+          auto load_q = [&](int t) {
+            if (k.n[t] == 0 || (nq[t] > 0 && !(ok = mbar_wait(&ms.q_free[t], (nq[t] - 1) & 1, wt, kSiteQFree, it)))) return;
+            mbar_arrive_expect_tx(&ms.q_full[t], kQTile);
+            for (int j = 0; j < 3; ++j)
+              tma_load_3d_hint(sbase + kOffQ + kQTile * t + kGranule * j, &map_q, 64 * j, k.head, k.q0 + kRows * t, &ms.q_full[t], once);
+            ++nq[t];
+          };
+          load_q(0);
           const int n = max(k.n[0], k.n[1]);
           for (int i = 0; i < n && ok; ++i) {
             const int at = k.k0 + (k.b0 + i) * kBlock;
@@ -527,6 +539,8 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
               uint64_t* bar = j < 3 ? &ms.k_full[b & 1] : &ms.v_full[b & 1];
               const uint32_t dst = sbase + kOffRing + (uint32_t)((kPerBlock * b + j) & 7) * kGranule;
               const int old = j < 3 ? b - 2 : b - 1;
+              if (i == 0 && j == 3) load_q(1);                // (the other tile can still be at work with its Q)
+              if (!ok) break;
               if (old >= 0 && j != 2 && j != 4) {
                 uint64_t* freed = j == 1 ? &ms.v_free[old & 1] : &ms.k_free[old & 1];
                 if (!(ok = mbar_wait(freed, (old >> 1) & 1, wt, kSiteEmpty, i))) break;
