@@ -616,27 +616,33 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         float4 mult[kSets];
 #pragma unroll
         for (int i = 0; i < kSets; ++i) mult[i] = scale[i];
+        // (groups 0 and 1, then the others: what is written for the tensor core has to be fenced before it is announced, and five fences
+        // a block took a quarter of the conversion's time)
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-          if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
+        for (int two = 0; two < 2; ++two) {
 #pragma unroll
-          for (int i = 0; i < kSets; ++i) {
-            const int r = kOwn * v + sub + 4 * i;
-            if (j < kGroups - 1) {
-              uint4 a, b;
-              convert16(codes[j % (kGroups - 1)][i], j == 0 ? mult[i].x : j == 1 ? mult[i].y : j == 2 ? mult[i].z : mult[i].w, a, b);
-              // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
-              const uint32_t base = slot + (2 * j + (c >> 2)) * kChunkBytes + r * 128, u = 2 * (c & 3), odd = c >> 2;
-              st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
-              st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
-            } else {
-              st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + ((c ^ (r & 7)) << 4), rope[i]);
+          for (int j = 2 * two; j < (two ? kGroups : 2); ++j) {
+            if (kb >= kSlots) ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)) && ok;
+#pragma unroll
+            for (int i = 0; i < kSets; ++i) {
+              const int r = kOwn * v + sub + 4 * i;
+              if (j < kGroups - 1) {
+                uint4 a, b;
+                convert16(codes[j % (kGroups - 1)][i], j == 0 ? mult[i].x : j == 1 ? mult[i].y : j == 2 ? mult[i].z : mult[i].w, a, b);
+                // lanes of odd chunks write their second half first: the eight lanes of a phase then cover all banks
+                const uint32_t base = slot + (2 * j + (c >> 2)) * kChunkBytes + r * 128, u = 2 * (c & 3), odd = c >> 2;
+                st_shared16(base + (((u + odd) ^ (r & 7)) << 4), odd ? b : a);
+                st_shared16(base + (((u + 1 - odd) ^ (r & 7)) << 4), odd ? a : b);
+              } else {
+                st_shared16(slot + (kChunks - 1) * kChunkBytes + r * 128 + ((c ^ (r & 7)) << 4), rope[i]);
+              }
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ms.kv_full[kb & 1][j]);
-          load(next, c1.n, j);
+          if (ok && lane < (two ? kGroups - 2 : 2)) mbar_arrive(&ms.kv_full[kb & 1][2 * two + lane]);
+#pragma unroll
+          for (int j = 2 * two; j < (two ? kGroups : 2); ++j) load(next, c1.n, j);
         }
         c0 = c1; c1 = c2; c2 = c3;
       }
