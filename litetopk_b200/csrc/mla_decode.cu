@@ -90,7 +90,7 @@ struct Params {
   uint32_t wait_limit;
 };
 
-enum { kSiteKv = 1, kSiteS, kSiteP, kSitePv, kSiteQ, kSiteFree };
+enum { kSiteKv = 1, kSiteS, kSiteP, kSitePv, kSiteQ, kSiteFree, kSiteVote, kSiteAlign };
 static __device__ int g_status[8];
 
 __device__ __forceinline__ bool elect_one() {
@@ -109,6 +109,12 @@ __device__ __forceinline__ bool softmax_any(bool x) {
                : "=r"(r) : "r"((uint32_t)x) : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -122,7 +128,8 @@ __device__ __forceinline__ int blocks_of(int len) { return max((len + kBlock - 1
 // Walks a CTA's share: blocks [k0, k1) of sequence b, piece by piece.
 struct Walk {
   int b, k0, k1, nb, len, left, index;
-  __device__ __forceinline__ Walk(const Misc& ms) : b(ms.start_b - 1), k0(0), k1(ms.start_k), nb(0), len(0), left(ms.count), index(-1) {}
+  template <class M>
+  __device__ __forceinline__ Walk(const M& ms) : b(ms.start_b - 1), k0(0), k1(ms.start_k), nb(0), len(0), left(ms.count), index(-1) {}
   __device__ __forceinline__ bool next(const Params& p) {
     if (left <= 0) return false;
     k0 = index < 0 ? k1 : 0;
@@ -135,6 +142,59 @@ struct Walk {
   }
   __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nb; }
 };
+
+// Group g's share: blocks [g total / groups, (g + 1) total / groups) of all sequences' in a row.  All threads of a block.
+template <class M>
+__device__ __forceinline__ void find_share(const Params& p, M& ms, int g, int warp, int lane) {
+  const int nt = (int)blockDim.x, per = (p.B + nt - 1) / nt;
+  const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += blocks_of(len_of(p, b));
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 31) ms.scan[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int before = incl - mine, total = 0;
+  for (int w = 0; w < nt / 32; ++w) {
+    if (w < warp) before += ms.scan[w];
+    total += ms.scan[w];
+  }
+  const int used = min(p.groups, total);
+  const int first = g < used ? (int)((long long)g * total / used) : total, last = g < used ? (int)((long long)(g + 1) * total / used) : total;
+  if (first >= before && first < before + mine && last > first) {
+    int at = before, b = b0;
+    for (;; ++b) {
+      const int nb = blocks_of(len_of(p, b));
+      if (first < at + nb) break;
+      at += nb;
+    }
+    ms.start_b = b; ms.start_k = first - at; ms.count = last - first;
+    ms.start_pos = first; ms.total = total; ms.meta_groups = used;
+  }
+  __syncthreads();
+}
+
+// which sequence of group g others have the rest of
+template <class M>
+__device__ __forceinline__ void write_meta(const Params& p, const M& ms, int g) {
+  int4 e = make_int4(-1, 0, 0, 0);
+  Walk w(ms);
+  int before = 0;
+  while (w.next(p)) {
+    if (w.k0 == 0 && w.k1 < w.nb) {
+      const long long end = ms.start_pos + before + w.nb;                 // behind the sequence's last block
+      e = make_int4(w.b, w.index == 0 ? 0 : 1, (int)((end * ms.meta_groups - 1) / ms.total) - g + 1, 0);
+    }
+    before += w.k1 - w.k0;
+  }
+  p.meta[g] = e;
+}
 
 // 16 e4m3 codes x scale -> 16 bf16
 __device__ __forceinline__ void convert16(const uint4& c, float scale, uint4& a, uint4& b) {
@@ -188,41 +248,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     tmem_relinquish_cta();
   }
   pdl_wait();
-  // This group's share: blocks [g total / groups, (g + 1) total / groups) of all sequences' in a row.
-  {
-    const int nt = (int)blockDim.x, per = (p.B + nt - 1) / nt;
-    const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += blocks_of(len_of(p, b));
-    int incl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += v;
-    }
-    if (lane == 31) ms.scan[warp] = incl;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    int before = incl - mine, total = 0;
-    for (int w = 0; w < nt / 32; ++w) {
-      if (w < warp) before += ms.scan[w];
-      total += ms.scan[w];
-    }
-    const int used = min(p.groups, total);
-    const int first = g < used ? (int)((long long)g * total / used) : total, last = g < used ? (int)((long long)(g + 1) * total / used) : total;
-    if (first >= before && first < before + mine && last > first) {
-      int at = before, b = b0;
-      for (;; ++b) {
-        const int nb = blocks_of(len_of(p, b));
-        if (first < at + nb) break;
-        at += nb;
-      }
-      ms.start_b = b; ms.start_k = first - at; ms.count = last - first;
-      ms.start_pos = first; ms.total = total; ms.meta_groups = used;
-    }
-    __syncthreads();
-  }
+  find_share(p, ms, g, warp, lane);
   const uint32_t tmem = __shfl_sync(0xffffffffu, ms.tmem_base, 0);
 
   if (warp < kSoftmaxWarps) {
@@ -294,10 +320,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] *= ms.corr[(c & (kRows - 1)) + e];
-              const uint32_t* r = reinterpret_cast<const uint32_t*>(o);
-              asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                           ::"r"(tmem + lane_base + c), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                             "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+              tmem_st16(tmem + lane_base + c, o);
             }
             tmem_wait_st();
           }
@@ -649,20 +672,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     }
   }
 
-  // which sequence of this group others have the rest of
-  if (warp == kWarpQk && rt == 0 && lane == 0 && p.meta) {
-    int4 e = make_int4(-1, 0, 0, 0);
-    Walk w(ms);
-    int before = 0;
-    while (w.next(p)) {
-      if (w.k0 == 0 && w.k1 < w.nb) {
-        const long long end = ms.start_pos + before + w.nb;               // behind the sequence's last block
-        e = make_int4(w.b, w.index == 0 ? 0 : 1, (int)((end * ms.meta_groups - 1) / ms.total) - g + 1, 0);
-      }
-      before += w.k1 - w.k0;
-    }
-    p.meta[g] = e;
-  }
+  if (warp == kWarpQk && rt == 0 && lane == 0 && p.meta) write_meta(p, ms, g);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -789,18 +799,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps, 3) mla_decode_merge_kernel(c
   }
 }
 
-static int rows_per_cta(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-struct Shape {
-  int per, tiles, groups;
-  Shape(int rows) {
-    per = rows_per_cta(rows);
-    tiles = (rows + per - 1) / per;
-    groups = min(max(1, sm_count() / tiles), 1024);
-  }
-  int64_t part_bytes() const { return (int64_t)groups * tiles * 2 * per * (kDV * 4 + 8); }
-  int64_t bytes() const { return groups == 1 ? 0 : part_bytes() + (int64_t)groups * 16; }
-};
-
 template <int kRows, Load kLoad>
 static int launch(const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
   if (!ensure_smem<mla_decode_kernel<kRows, kLoad>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
@@ -815,9 +813,34 @@ static int launch(Load l, const CUtensorMap& map, const CUtensorMap& map_q, cons
 }  // namespace decode
 }  // namespace lt
 
+#include "mla_decode_pair.cuh"
+
+namespace lt {
+namespace decode {
+
+// Up to 32 rows a CTA has a tile, more have pairs of CTAs.
+struct Shape {
+  int per, tiles, groups;
+  Shape(int rows, Load l) {
+    per = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    tiles = (rows + per - 1) / per;
+    const int units = per <= 32 ? sm_count()
+                      : per == 64 ? (l == kTma ? pair::pairs<32, kTma>() : l == kCopy ? pair::pairs<32, kCopy>() : pair::pairs<32, kPacked>())
+                                  : (l == kTma ? pair::pairs<64, kTma>() : l == kCopy ? pair::pairs<64, kCopy>() : pair::pairs<64, kPacked>());
+    groups = min(max(1, units / tiles), kMaxGroups);
+  }
+  int64_t part_bytes() const { return (int64_t)groups * tiles * 2 * per * (kDV * 4 + 8); }
+  int64_t bytes() const { return groups == 1 ? 0 : part_bytes() + (int64_t)groups * 16; }
+};
+// What a workspace has to hold does not depend on how rows are loaded, as a caller does not know that.
+static int64_t workspace(int rows) { return max(Shape(rows, kTma).bytes(), max(Shape(rows, kCopy).bytes(), Shape(rows, kPacked).bytes())); }
+
+}  // namespace decode
+}  // namespace lt
+
 extern "C" int64_t litedsa_mla_decode_workspace(int q_len, int heads) {
   if (q_len <= 0 || heads <= 0 || heads > 128 || (int64_t)q_len * heads > (1 << 20)) return 0;
-  return lt::decode::Shape(q_len * heads).bytes();
+  return lt::decode::workspace(q_len * heads);
 }
 
 extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -837,8 +860,10 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
       (q_batch_stride | q_token_stride | q_head_stride) % 8 || ((uintptr_t)lse & 3))
     return LITEDSA_ERR_UNSUPPORTED;
   if (B == 0) return LITEDSA_OK;
-  const Shape s(q_len * heads);
-  if (s.bytes() > 0 && (!workspace || workspace_bytes < s.bytes())) return workspace ? LITEDSA_ERR_SHAPE : LITEDSA_ERR_ARG;
+  const Load load = packed ? kPacked : block_size % (q_len * heads <= 32 ? kBlock : pair::kOwnKeys) == 0 ? kTma : kCopy;
+  const Shape s(q_len * heads, load);
+  const int64_t need = decode::workspace(q_len * heads);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return workspace ? LITEDSA_ERR_SHAPE : LITEDSA_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   Params p = {};
   p.q = reinterpret_cast<const uint8_t*>(q);
@@ -856,19 +881,19 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   p.scale_log2 = sm_scale * kLog2e;
   p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
   CUtensorMap map = {};
-  const Load load = packed ? kPacked : block_size % kBlock == 0 ? kTma : kCopy;
   if (load == kTma && n_blocks > 0 &&
       !make_map_3d(&map, cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)block_size, (uint64_t)n_blocks, 2 * kD,
-                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, kBlock, 1))
+                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, s.per <= 32 ? kBlock : pair::kOwnKeys, 1))
     return LITEDSA_ERR_CUDA;
   // Rows (token, head) of a sequence that are evenly spaced (one token, or no gap behind a token's heads) are a matrix.
   CUtensorMap map_q = {};
   p.flat_q = q_len == 1 || q_token_stride == heads * q_head_stride;
   const int64_t row_stride = heads > 1 ? q_head_stride : q_len > 1 ? q_token_stride : kD;
   if (p.flat_q && !make_map_3d(&map_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)p.rows, (uint64_t)B, (uint64_t)(2 * row_stride),
-                               (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)s.per, 1))
+                               (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)(s.per <= 32 ? s.per : s.per / 2), 1))
     p.flat_q = 0;                                                          // (a stride of 0, for one, is no map's)
-  const int rc = s.per == 16 ? launch<16>(load, map, map_q, p, st) : s.per == 32 ? launch<32>(load, map, map_q, p, st) : launch<64>(load, map, map_q, p, st);
+  const int rc = s.per == 16 ? launch<16>(load, map, map_q, p, st) : s.per == 32 ? launch<32>(load, map, map_q, p, st)
+                 : s.per == 64 ? pair::launch<32>(load, map, map_q, p, st) : pair::launch<64>(load, map, map_q, p, st);
   if (rc != LITEDSA_OK || s.groups == 1) return rc;
   const int64_t most = (int64_t)min(B, s.groups) * p.rows;                 // rows that can need it
   return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)min(most, (int64_t)3 * sm_count())), 32 * kMergeWarps, 0, st, p, s.per);
