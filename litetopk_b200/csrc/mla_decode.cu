@@ -84,13 +84,13 @@ struct Params {
   float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
   int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
   int flat_q;                     // a sequence's rows are evenly spaced: they come by TMA
-  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks;
+  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows;      // box_rows: of a pair's loads
   float scale_log2;
   int epoch;
   uint32_t wait_limit;
 };
 
-enum { kSiteKv = 1, kSiteS, kSiteP, kSitePv, kSiteQ, kSiteFree, kSiteVote, kSiteAlign };
+enum { kSiteKv = 1, kSiteS, kSiteP, kSitePv, kSiteQ, kSiteFree, kSiteVote, kSiteAid, kSiteAlign };
 static __device__ int g_status[8];
 
 __device__ __forceinline__ bool elect_one() {
@@ -102,6 +102,29 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// The page and the row in it of a key that moves on by a block at a time: a division took a loading warp 200 cycles, five a block.
+struct PageAt {
+  int size, add_page, add_row, page, row;
+  __device__ __forceinline__ explicit PageAt(int block_size) : size(block_size), add_page(kBlock / block_size), page(0), row(0) { add_row = kBlock - add_page * size; }
+  __device__ __forceinline__ void at(int key) {
+    page = key / size;
+    row = key - page * size;
+  }
+  __device__ __forceinline__ void advance() {
+    page += add_page;
+    row += add_row;
+    if (row >= size) { row -= size; ++page; }
+  }
+};
+// true once in `every` calls, the first time after `from` of them
+struct Turn {
+  int every, left;
+  __device__ __forceinline__ bool operator()() {
+    if (left-- > 0) return false;
+    left = every - 1;
+    return true;
+  }
+};
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool softmax_any(bool x) {
   uint32_t r;
@@ -141,6 +164,61 @@ struct Walk {
     return true;
   }
   __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == nb; }
+};
+
+// Where a loading warp's rows of a block lie, for the blocks that it comes to: lane i has those of the i-th from the last look on.  Looked up thirty
+// at a time: a look and its divisions a block took such a warp 400 to 1000 cycles, a third of what a block takes.
+template <bool kTwo>
+struct Ahead {
+  Walk w;
+  int at, i, offset, own;                                   // rows [offset, offset + own) of each block
+  bool more;
+  int page, row, n, page2;                                  // n of them hold keys; n_blocks: a page beyond the cache, or none; page2: of rows from 16 on
+  template <class M>
+  __device__ __forceinline__ Ahead(const M& ms, const Params& p, int first, int rows, int lane) : w(ms), i(0), offset(first), own(rows), page(0), row(0), n(0), page2(0) {
+    more = w.next(p);
+    at = w.k0;
+    fill(p, 0, lane);
+  }
+  __device__ __forceinline__ void fill(const Params& p, int filled, int lane) {
+    if (lane >= filled) { page = page2 = p.n_blocks; row = n = 0; }
+    while (more && filled < 32) {
+      const int take = min(32 - filled, w.k1 - at);
+      if (lane >= filled && lane < filled + take) {
+        const int key = (at + lane - filled) * kBlock + offset;
+        n = min(max(w.len - key, 0), own);
+        if (n > 0) {
+          const int c = key / p.block_size;
+          const int* from = p.table + w.b * p.table_pitch + c;
+          row = key - c * p.block_size;
+          page = __ldcg(from);
+          if ((unsigned)page >= (unsigned)p.n_blocks) page = p.n_blocks;
+          if (kTwo) {
+            page2 = n > 16 && row + 16 >= p.block_size ? __ldcg(from + 1) : page;
+            if ((unsigned)page2 >= (unsigned)p.n_blocks) page2 = p.n_blocks;
+          }
+        }
+      }
+      filled += take;
+      at += take;
+      if (at == w.k1) { more = w.next(p); at = w.k0; }
+    }
+  }
+  __device__ __forceinline__ void advance(const Params& p, int lane) {
+    if (++i < 30) return;
+    page = __shfl_down_sync(0xffffffffu, page, 30);
+    row = __shfl_down_sync(0xffffffffu, row, 30);
+    n = __shfl_down_sync(0xffffffffu, n, 30);
+    if (kTwo) page2 = __shfl_down_sync(0xffffffffu, page2, 30);
+    i = 0;
+    fill(p, 2, lane);
+  }
+  // of the block d = 0, 1, 2 from the current one
+  __device__ __forceinline__ int rows_in(int d) const { return __shfl_sync(0xffffffffu, n, i + d); }
+  __device__ __forceinline__ const uint8_t* rows_of(const Params& p, int d, int row_bytes) const {           // none: nullptr
+    const int x = __shfl_sync(0xffffffffu, page, i + d), r = __shfl_sync(0xffffffffu, row, i + d);
+    return x < p.n_blocks ? p.cache + (long long)x * p.block_pitch + (long long)r * row_bytes : nullptr;
+  }
 };
 
 // Group g's share: blocks [g total / groups, (g + 1) total / groups) of all sequences' in a row.  All threads of a block.
@@ -505,45 +583,30 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
   } else if (kLoad == kTma) {
    if (warp == kWarpTma) {
     // ------------------------------------------------------------ bf16 rows by TMA: a block is of one page, nine boxes of 64 dims
-    // All lanes keep the pages of the blocks under way, of which the furthest, two ahead of the one requested, is brought into L2: the
-    // load that follows a freed slot then takes L2's latency.
-    struct Coming { int page, row; };                                     // page -1: no block, or one without keys
-    Walk w(ms);
+    // The block two ahead of the one requested is brought into L2: the load that follows a freed slot then takes L2's latency.
     const int count = ms.count;
-    int at = 0, looked = 0;
-    if (w.next(p)) at = w.k0;
-    auto look = [&]() -> Coming {
-      Coming c{-1, 0};
-      if (looked >= count) return c;
-      const int key = at * kBlock;
-      c.row = key % p.block_size;
-      if (key < w.len) {
-        c.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
-        if ((unsigned)c.page >= (unsigned)p.n_blocks) c.page = p.n_blocks;                        // beyond the cache: reads as zeros
-      }
-      ++looked;
-      if (++at == w.k1 && w.next(p)) at = w.k0;
-      return c;
-    };
+    Ahead<false> next(ms, p, 0, kBlock, lane);
+    Turn mine_to_bring{p.row_tiles, rt};
     const uint64_t pol = l2_policy_evict_first();
     const uint32_t mine = sbase + PL::kOffKV + lane * kChunkBytes;
     int asked = 0;
     bool ok = true;
-    Coming c0 = look(), c1 = look(), c2 = look();
-    for (int kb = 0; ok && kb < count; ++kb) {
-      const Coming c3 = look();
+    for (int kb = 0; ok && kb < count; ++kb, next.advance(p, lane)) {
+      const int page = __shfl_sync(0xffffffffu, next.page, next.i), row = __shfl_sync(0xffffffffu, next.row, next.i);
+      const bool some = next.rows_in(0) > 0;
 #pragma unroll 1
       for (int j = 0; j < kGroups; ++j) {
         if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
-        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1][j], c0.page >= 0 ? (j < kGroups - 1 ? 2 : 1) * kChunkBytes : 0u);
+        if (lane == 0) mbar_arrive_expect_tx(&ms.kv_full[kb & 1][j], some ? (j < kGroups - 1 ? 2 : 1) * kChunkBytes : 0u);
         __syncwarp();
-        if (c0.page >= 0 && (lane >> 1) == j && lane < kChunks)
-          tma_load_3d_hint(mine + (kb & 1) * kSlotBytes, &map_kv, 64 * lane, c0.row, c0.page, &ms.kv_full[kb & 1][j], pol);
+        if (some && (lane >> 1) == j && lane < kChunks)
+          tma_load_3d_hint(mine + (kb & 1) * kSlotBytes, &map_kv, 64 * lane, row, page, &ms.kv_full[kb & 1][j], pol);
         asked = kGroups * kb + j + 1;
       }
-      if (lane == 0 && c2.page >= 0 && c2.page < p.n_blocks && (looked + rt) % p.row_tiles == 0)
-        l2_prefetch_1d(p.cache + (long long)c2.page * p.block_pitch + (long long)c2.row * (2 * kD), kBlock * 2 * kD);
-      c0 = c1; c1 = c2; c2 = c3;
+      if (mine_to_bring()) {
+        const uint8_t* src = next.rows_of(p, 2, 2 * kD);
+        if (src != nullptr && lane == 0) l2_prefetch_1d(src, kBlock * 2 * kD);
+      }
     }
     if (!ok)                                                              // given up: what is in flight lands first
       for (int i = max(asked - kSlots * kGroups, 0); i < asked; ++i) {
@@ -561,18 +624,25 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     Walk w(ms);
     const int count = ms.count;
     int at = 0, looked = 0;
-    if (w.next(p)) at = w.k0;
+    PageAt pa(p.block_size);
+    auto piece = [&]() {
+      if (!w.next(p)) return;
+      at = w.k0;
+      pa.at(at * kBlock + kOwn * v);
+    };
+    piece();
     auto look = [&]() -> Coming {
       Coming x{-1, 0, 0};
       if (looked >= count) return x;
-      const int key = at * kBlock + kOwn * v;
-      x.n = min(max(w.len - key, 0), kOwn);
-      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
-      x.row = key % p.block_size;
+      x.n = min(max(w.len - at * kBlock - kOwn * v, 0), kOwn);
+      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + pa.page);
+      x.row = pa.row;
       ++looked;
-      if (++at == w.k1 && w.next(p)) at = w.k0;
+      pa.advance();
+      if (++at == w.k1) piece();
       return x;
     };
+    Turn mine_to_bring{p.row_tiles, rt};
     auto rows_of = [&](const Coming& x) -> const uint8_t* {
       return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kRowBytes : nullptr;
     };
@@ -581,15 +651,15 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       if (src != nullptr && lane == 0) l2_prefetch_1d(src, (uint32_t)(x.n * kRowBytes));
     };
     bool ok = true;
-    Coming c0 = look(), c1 = look(), c2 = look();
-    to_l2(c0);
+    Coming c0, c1 = look(), c2 = look(), c3 = look();
     to_l2(c1);
+    to_l2(c2);
     if (kLoad == kCopy) {
       for (int kb = 0; ok && kb < count; ++kb) {
-        const Coming c3 = look();
+        c0 = c1; c1 = c2; c2 = c3; c3 = look();
         const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
         const uint8_t* src = rows_of(c0);
-        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
+        if (mine_to_bring()) to_l2(c2);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
           if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
@@ -604,7 +674,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
           }
           cp_async_mbar_arrive_noinc(&ms.kv_full[kb & 1][j]);
         }
-        c0 = c1; c1 = c2; c2 = c3;
       }
       cp_async_wait_all();
     } else {
@@ -627,15 +696,15 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         }
       };
       {
-        const uint8_t* src = rows_of(c0);
+        const uint8_t* src = rows_of(c1);
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) load(src, c0.n, j);
+        for (int j = 0; j < kGroups; ++j) load(src, c1.n, j);
       }
       for (int kb = 0; ok && kb < count; ++kb) {
-        const Coming c3 = look();
+        c0 = c1; c1 = c2; c2 = c3; c3 = look();
         const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
         const uint8_t* next = rows_of(c1);
-        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
+        if (mine_to_bring()) to_l2(c2);
         float4 mult[kSets];
 #pragma unroll
         for (int i = 0; i < kSets; ++i) mult[i] = scale[i];
@@ -667,7 +736,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
 #pragma unroll
           for (int j = 2 * two; j < (two ? kGroups : 2); ++j) load(next, c1.n, j);
         }
-        c0 = c1; c1 = c2; c2 = c3;
       }
     }
   }
@@ -818,22 +886,22 @@ static int launch(Load l, const CUtensorMap& map, const CUtensorMap& map_q, cons
 namespace lt {
 namespace decode {
 
-// Up to 32 rows a CTA has a tile, more have pairs of CTAs.
+// Up to 64 rows a CTA has a tile, more have pairs of CTAs, 128 rows a pair.  (32 sequences of up to 8191 packed rows, 64 heads: 61 us against 67 with pairs of
+// 32 rows a CTA; 256 rows, bf16: 115 against 133 with four CTAs of 64; 128 sequences of 128 heads, packed: 160 against 215.)
 struct Shape {
   int per, tiles, groups;
-  Shape(int rows, Load l) {
+  bool pair;
+  Shape(int rows, Load l) : pair(rows > 64) {
     per = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     tiles = (rows + per - 1) / per;
-    const int units = per <= 32 ? sm_count()
-                      : per == 64 ? (l == kTma ? pair::pairs<32, kTma>() : l == kCopy ? pair::pairs<32, kCopy>() : pair::pairs<32, kPacked>())
-                                  : (l == kTma ? pair::pairs<64, kTma>() : l == kCopy ? pair::pairs<64, kCopy>() : pair::pairs<64, kPacked>());
+    const int units = !pair ? sm_count() : l == kPacked ? decode::pair::pairs<kPacked>() : decode::pair::pairs<kTma>();
     groups = min(max(1, units / tiles), kMaxGroups);
   }
   int64_t part_bytes() const { return (int64_t)groups * tiles * 2 * per * (kDV * 4 + 8); }
   int64_t bytes() const { return groups == 1 ? 0 : part_bytes() + (int64_t)groups * 16; }
 };
 // What a workspace has to hold does not depend on how rows are loaded, as a caller does not know that.
-static int64_t workspace(int rows) { return max(Shape(rows, kTma).bytes(), max(Shape(rows, kCopy).bytes(), Shape(rows, kPacked).bytes())); }
+static int64_t workspace(int rows) { return max(Shape(rows, kTma).bytes(), Shape(rows, kPacked).bytes()); }
 
 }  // namespace decode
 }  // namespace lt
@@ -860,7 +928,7 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
       (q_batch_stride | q_token_stride | q_head_stride) % 8 || ((uintptr_t)lse & 3))
     return LITEDSA_ERR_UNSUPPORTED;
   if (B == 0) return LITEDSA_OK;
-  const Load load = packed ? kPacked : block_size % (q_len * heads <= 32 ? kBlock : pair::kOwnKeys) == 0 ? kTma : kCopy;
+  const Load load = packed ? kPacked : q_len * heads > 64 || block_size % kBlock == 0 ? kTma : kCopy;
   const Shape s(q_len * heads, load);
   const int64_t need = decode::workspace(q_len * heads);
   if (need > 0 && (!workspace || workspace_bytes < need)) return workspace ? LITEDSA_ERR_SHAPE : LITEDSA_ERR_ARG;
@@ -878,22 +946,23 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   }
   p.B = B; p.q_len = q_len; p.heads = heads; p.rows = q_len * heads; p.row_tiles = s.tiles; p.groups = s.groups;
   p.cols = n_blocks == 0 ? 0 : table_cols; p.block_size = block_size; p.n_blocks = (int)n_blocks;
+  p.box_rows = block_size % pair::kOwnKeys == 0 ? pair::kOwnKeys : 16;
   p.scale_log2 = sm_scale * kLog2e;
   p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
   CUtensorMap map = {};
   if (load == kTma && n_blocks > 0 &&
       !make_map_3d(&map, cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)block_size, (uint64_t)n_blocks, 2 * kD,
-                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, s.per <= 32 ? kBlock : pair::kOwnKeys, 1))
+                   (uint64_t)(n_blocks > 1 ? block_stride_bytes : (int64_t)block_size * row), 64, s.pair ? (uint32_t)p.box_rows : (uint32_t)kBlock, 1))
     return LITEDSA_ERR_CUDA;
   // Rows (token, head) of a sequence that are evenly spaced (one token, or no gap behind a token's heads) are a matrix.
   CUtensorMap map_q = {};
   p.flat_q = q_len == 1 || q_token_stride == heads * q_head_stride;
   const int64_t row_stride = heads > 1 ? q_head_stride : q_len > 1 ? q_token_stride : kD;
   if (p.flat_q && !make_map_3d(&map_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kD, (uint64_t)p.rows, (uint64_t)B, (uint64_t)(2 * row_stride),
-                               (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)(s.per <= 32 ? s.per : s.per / 2), 1))
+                               (uint64_t)(2 * (B > 1 ? q_batch_stride : kD)), 64, (uint32_t)(s.pair ? s.per / 2 : s.per), 1))
     p.flat_q = 0;                                                          // (a stride of 0, for one, is no map's)
   const int rc = s.per == 16 ? launch<16>(load, map, map_q, p, st) : s.per == 32 ? launch<32>(load, map, map_q, p, st)
-                 : s.per == 64 ? pair::launch<32>(load, map, map_q, p, st) : pair::launch<64>(load, map, map_q, p, st);
+                 : s.per == 64 ? launch<64>(load, map, map_q, p, st) : pair::launch(load, map, map_q, p, st);
   if (rc != LITEDSA_OK || s.groups == 1) return rc;
   const int64_t most = (int64_t)min(B, s.groups) * p.rows;                 // rows that can need it
   return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)min(most, (int64_t)3 * sm_count())), 32 * kMergeWarps, 0, st, p, s.per);

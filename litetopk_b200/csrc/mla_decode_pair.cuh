@@ -11,8 +11,9 @@
 // that is the peer's dims.  Either way keys 0-31 then lie in chunks 0-3 and keys 32-63 in chunks 4-7.  P takes the place of the rope dims.
 // Both products are issued in the leader (CTA 0).  S has keys 0-31 in lanes 0-63 and keys 32-63 in lanes 64-127, a row a lane.
 //
-// O's columns are the rows of both CTAs, so a rescaling is the business of both: each block they tell each other whether one of
-// their rows needs it, which is hidden by the blocks in flight, and it is rare: P may be 2^32 above the running maximum (mla_prefill.cu).
+// O's columns are the rows of both CTAs, so a rescaling is the business of both, and rare: P may be 2^32 above the running maximum
+// (mla_prefill.cu).  A CTA whose rows need one has four warps of the other do their part and holds its P back until that is
+// done; asking each other every block took 1600 cycles of it.
 #pragma once
 
 namespace lt {
@@ -20,59 +21,98 @@ namespace decode {
 namespace pair {
 
 constexpr int kOwnKeys = 32;
+constexpr uint32_t kMiscBytes = 3 * 1024;
 constexpr uint32_t kChunk = kOwnKeys * 128;                 // 32 keys x 64 bf16
 constexpr uint32_t kSlot = kChunks * kChunk;
-constexpr int kWarpK = 11, kWarpV = 12, kLoad0 = 12;        // kTma: two warps; else K and V have half of the warps from kLoad0 each
-template <Load kLoad> constexpr int kLoaders = kLoad == kTma ? 1 : kLoad == kCopy ? 8 : 16;
-template <Load kLoad> constexpr int kPairThreads = 32 * (kLoad0 + kLoaders<kLoad>);
+// Warps 0-7: softmax; 8, 9: products; 10: queries.  kTma: 11 and 13 request keys (the issue of small boxes paces a warp), 12 values; kPacked:
+// 11 brings keys into L2, 12-19 convert keys, 20-23 values.  The last four: the other CTA's rescalings.
+constexpr int kWarpK0 = 11, kWarpV = 12, kWarpK1 = 13, kWarpBring = 11, kLoad0 = 12, kKeyWarps = 8, kValueWarps = 4;
+template <Load kLoad> constexpr int kWarpAid = kLoad == kTma ? 16 : 24;
+template <Load kLoad> constexpr int kPairThreads = 32 * (kWarpAid<kLoad> + 4);
 constexpr float kMostOver = 32.f;
+constexpr int R = 64;                                       // rows of a CTA
 
-template <int R>
-struct PairPlan {
-  static constexpr int kSlots = R == 64 ? 4 : 5;
+struct PL {
+  static constexpr int kSlots = 4;
   static constexpr uint32_t kQChunk = R * 128;
   static constexpr uint32_t kOffKV = 0;
   static constexpr uint32_t kOffQ = kOffKV + kSlots * kSlot;
-  static constexpr uint32_t kOffP = kOffQ + kChunks * kQChunk;              // R = 64: keys 32-63 of P, two buffers; keys 0-31 fill the rope chunk
+  static constexpr uint32_t kOffP = kOffQ + kChunks * kQChunk;              // keys 32-63 of P, two buffers; keys 0-31 fill the rope chunk
   static constexpr uint32_t kPHalf = R * kOwnKeys * 2;
-  static constexpr uint32_t kOffMisc = kOffP + (R == 64 ? 2 * kPHalf : 4096);      // (R = 32: the 64 rows of the operand end in there)
-  static constexpr uint32_t kSmem = kOffMisc + 3072;
+  static constexpr uint32_t kOffMisc = kOffP + 2 * kPHalf;
+  static constexpr uint32_t kSmem = kOffMisc + kMiscBytes;
   static constexpr uint32_t kTmemS = 4 * R;                 // O^T: two blocks of 2 R columns; then S, 32 columns a slot
   static constexpr uint32_t kTmemCols = 512;
   static_assert(kOffQ % 1024 == 0 && kSlot % 1024 == 0 && kOffP % 1024 == 0, "swizzled tiles");
-  static_assert(kOffQ + (kChunks - 1) * kQChunk + 64 * 128 <= kOffMisc, "the operand ends inside");
   static_assert(kTmemS + 32 * kSlots <= kTmemCols, "tensor memory");
   static_assert(kSmem <= 232448, "shared memory");
 };
 
 struct PairMisc {
   // in the leader: what the products wait for, from both CTAs
-  uint64_t k_full[5], v_full[5], p_ready[5], q_ready;
+  uint64_t k_full[4], v_full[4], p_ready[4], q_ready;
   // in each CTA
-  uint64_t qk_done[5], slot_free[5], q_free, drained[2], vote[2], corr_full, fin_full;
-  uint32_t vote_flag[2];
+  uint64_t qk_done[4], slot_free[4], q_free, drained[2], asked, answered, fin_full;
+  uint64_t decided;                   // a block's maxima are settled
+  uint32_t changes, asks;             // how often they changed; how often the peer was asked to rescale
+  uint32_t asked_slot, asked_phase, over;      // of the block whose products are in O; no more will be asked
   uint32_t left, tmem_base;
   int start_b, start_k, count, meta_groups;
   long long start_pos, total;
   int scan[32];
-  float top[4][64];                   // of a row's four threads: maxima, sums
-  float corr[128], scale[128];        // of the tile's rows
+  float top[4][64];                   // of a row's threads: maxima, sums
+  float most[64];                     // what the rows' exponentials are relative to
+  float corr[64], corr_peer[64];      // factors of this CTA's and of the peer's rows
+  float scale[128];                   // of the tile's rows
 };
-static_assert(sizeof(PairMisc) <= 3072, "PairMisc");
+static_assert(sizeof(PairMisc) <= kMiscBytes, "PairMisc");
 
+// (relaxed: nothing that this thread has written is announced, and a release waited a thousand cycles for its prefetches)
 __device__ __forceinline__ void arrive_expect_cluster(uint32_t addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes) : "memory");
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ uint32_t try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendHintNs) : "memory");
+  return ok;
+}
 // a wait for what the other CTA has written
 __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, const BlockWaiter& w, int site, int iter) {
-  uint32_t since = 0, ok;
-  for (;;) {
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendHintNs) : "memory");
-    if (ok) return true;
+  uint32_t since = 0;
+  while (!try_wait_cluster(bar, parity))
     if (w.gives_up(since, site, iter)) return false;
+  return true;
+}
+// a vote among the four warps of a softmax group
+__device__ __forceinline__ bool group_any(int group, bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((uint32_t)x), "r"(3 + group) : "memory");
+  return r != 0;
+}
+// and of the four that rescale for the peer
+__device__ __forceinline__ bool aid_any(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((uint32_t)x) : "memory");
+  return r != 0;
+}
+// R columns of this warp's 32 lanes, column x by factor x
+__device__ __forceinline__ void rescale(uint32_t taddr, const float* factors) {
+  tc_fence_after();
+#pragma unroll 1
+  for (int x = 0; x < R; x += 16) {
+    float o[16];
+    tmem_ld16(taddr + x, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] *= factors[x + e];
+    tmem_st16(taddr + x, o);
   }
+  tmem_wait_st();
+  tc_fence_before();
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void commit_pair(uint32_t addr) {
@@ -99,9 +139,6 @@ __device__ __forceinline__ void mma2_pair(uint32_t d, uint32_t a_lo, uint32_t a_
       ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate_first), "n"(kDa), "n"(kDb) : "memory");
 }
 
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-
 // a running block's slot and the parity of its barriers
 template <int kSlots>
 struct Ring {
@@ -112,10 +149,9 @@ struct Ring {
   }
 };
 
-template <int R, Load kLoad>
+template <Load kLoad>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads<kLoad>, 1)
 mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q, const Params p) {
-  using PL = PairPlan<R>;
   constexpr int kSlots = PL::kSlots, kTile = 2 * R;
   using Cursor = Ring<kSlots>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -133,19 +169,22 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
   const int cluster = (int)blockIdx.x >> 1, g = cluster / p.row_tiles, rt = cluster - g * p.row_tiles;
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 5; ++i) {
-      // arrivals of both CTAs: a loader warp each with its bytes; the threads' own copies; the converting warps
-      mbar_init(&ms.k_full[i], kLoad == kTma ? 2 : kLoaders<kLoad>);
-      mbar_init(&ms.v_full[i], kLoad == kTma ? 2 : kLoaders<kLoad>);
-      mbar_init(&ms.p_ready[i], 2 * kSoftmaxWarps);
+    for (int i = 0; i < PL::kSlots; ++i) {
+      // warps of both CTAs
+      mbar_init(&ms.k_full[i], 2 * (kLoad == kTma ? 2 : kKeyWarps));
+      mbar_init(&ms.v_full[i], 2 * (kLoad == kTma ? 1 : kValueWarps));
+      mbar_init(&ms.p_ready[i], 2);
       mbar_init(&ms.qk_done[i], 1);
       mbar_init(&ms.slot_free[i], 1);
     }
     mbar_init(&ms.q_ready, 2);
     mbar_init(&ms.q_free, 1);
-    mbar_init(&ms.corr_full, 1);
+    mbar_init(&ms.asked, 1);
+    mbar_init(&ms.answered, 1);
+    mbar_init(&ms.decided, 1);
+    ms.over = ms.changes = ms.asks = 0;
     mbar_init(&ms.fin_full, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&ms.drained[i], 1); mbar_init(&ms.vote[i], 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(&ms.drained[i], 1);
     ms.left = 0;
     ms.count = 0;
     fence_mbar_init();
@@ -165,119 +204,146 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax, epilogue
-    // Warp: TMEM lanes 32 (warp % 4), columns 16 (warp / 4).  Thread: row r, keys 32 h + 16 c + [0, 16).
+    // Two groups of four warps take turns, a block each: warp (warp % 4) has TMEM lanes 32 (warp % 4), a thread row r and keys 32 h + [0, 32).
+    // Blocks' maxima are settled in order (decided): whoever finds a row past its bound changes the row's for both groups, which
+    // the other sees before it hands its P over.
     const int quarter = warp & 3, c = warp >> 2, tl = 32 * quarter + lane, r = tl & 63, h = tl >> 6;
-    const bool live = (quarter & 1) * 32 < R;
     const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
     const uint32_t a_p_ready = mapa(smem_u32(&ms.p_ready[0]), 0);
-    const uint32_t a_vote = mapa(smem_u32(&ms.vote[0]), peer), a_flag = mapa(smem_u32(&ms.vote_flag[0]), peer);
+    volatile uint32_t* const changes = &ms.changes;
+    volatile uint32_t* const asks = &ms.asks;
     Walk w(ms);
     Cursor at, prev, prev2;                                 // of blocks kb, kb - 1, kb - 2
     int kb = 0;
-    uint32_t corrs = 0;                                     // rescalings so far
+    uint32_t seen = 0;                                      // changes
     // A wait here that gives up is passed like any other: the warps meet at named barriers, so they take the same steps.
     bool more = w.next(p);
     while (more) {
       const int row = row0 + r;
       const int lim = min(w.len, w.len - p.q_len + 1 + row / p.heads), low = w.len - p.q_len + 1 + row0 / p.heads;     // low: what this CTA's first row sees
       float m = kMInit, l = 0.f;
-      for (int k = w.k0; k < w.k1; ++k, ++kb) {
+      auto renew = [&]() -> bool {                          // have the maxima changed?
+        if (*changes == seen) return false;
+        seen = *changes;
+        const float now = ms.most[r];
+        l *= fast_exp2(m - now);
+        m = now;
+        return true;
+      };
+      for (int k = w.k0; k < w.k1; ++k, ++kb, prev2 = prev, prev = at, at.advance()) {
+        if ((kb & 1) != c) continue;
         mbar_wait(&ms.qk_done[at.slot], at.phase, wt, kSiteS, kb);
         __syncwarp();
         tc_fence_after();
-        float v[16];
+        float v[32];
         float mx = -INFINITY;
-        if (live) {
-          tmem_ld16(tmem + PL::kTmemS + 32 * at.slot + 16 * c + lane_base, v);
-          tmem_wait_ld();
-          if ((k + 1) * kBlock > low) {
-            const int seen = lim - k * kBlock - 32 * h - 16 * c;
+        tmem_ld32(tmem + PL::kTmemS + 32 * at.slot + lane_base, v);
+        tmem_wait_ld();
+        if ((k + 1) * kBlock > low) {
+          const int keys = lim - k * kBlock - 32 * h;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = e < seen ? v[e] * p.scale_log2 : -INFINITY;
-          } else {
+          for (int e = 0; e < 32; ++e) v[e] = e < keys ? v[e] * p.scale_log2 : -INFINITY;
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= p.scale_log2;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, v[e]);
+          for (int e = 0; e < 32; ++e) v[e] *= p.scale_log2;
         }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, v[e]);
         const bool first = k == w.k0;
-        const bool mine = softmax_any(mx > m + kMostOver);
-        // whether one of the pair's rows needs it
-        if (threadIdx.x == 0) {
-          st_cluster_u32(a_flag + 4u * (kb & 1), mine ? 1u : 0u);
-          mbar_arrive_cluster_release(a_vote + 8u * (kb & 1));
+        if (k == w.k0 + 1) {                                // (a piece's first block changes them)
+          mbar_wait(&ms.decided, (kb - 1) & 1, wt, kSiteVote, kb);
+          __syncwarp();
+          renew();
         }
-        wait_cluster(&ms.vote[kb & 1], (kb >> 1) & 1, wt, kSiteVote, kb);
-        // (put to the vote among the threads once more: a wait that gave up must not part them)
-        if (softmax_any(first || mine || *reinterpret_cast<volatile uint32_t*>(&ms.vote_flag[kb & 1]) != 0)) {
-          if (live) ms.top[2 * c + h][r] = mx;
-          softmax_sync();
-          float f = 1.f;
-          if (live) {
-            const float now = fmaxf(m, fmaxf(fmaxf(ms.top[0][r], ms.top[1][r]), fmaxf(ms.top[2][r], ms.top[3][r])));
-            f = fast_exp2(m - now);
-            m = now;
-            l *= f;
-          }
-          if (!first) {
-            // the factors of all of the tile's rows, in both CTAs
-            if (live && h == 0 && c == 0) {
-              ms.corr[R * cta + r] = f;
-              st_cluster_f32(mapa(smem_u32(&ms.corr[R * cta + r]), peer), f);
-            }
-            fence_cluster();
-            softmax_sync();
-            if (threadIdx.x == 0) mbar_arrive_cluster_release(mapa(smem_u32(&ms.corr_full), peer));
-            wait_cluster(&ms.corr_full, corrs & 1, wt, kSiteVote, kb);
-            ++corrs;
-            mbar_wait(&ms.slot_free[prev.slot], prev.phase, wt, kSitePv, kb);
-            __syncwarp();
-            tc_fence_after();
-#pragma unroll 1
-            for (int x = kTile * c; x < kTile * (c + 1); x += 16) {
-              float o[16];
-              tmem_ld16(tmem + lane_base + x, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= ms.corr[(x & (kTile - 1)) + e];
-              tmem_st16(tmem + lane_base + x, o);
-            }
-            tmem_wait_st();
-          }
-        }
-        if (R == 64 && kb >= 2) {                           // this buffer's last P has been read
+        auto must = [&]() { return first || __any_sync(0xffffffffu, mx > m + kMostOver); };
+        const bool need = must();
+        if (kb >= 2) {                                      // this buffer's last P has been read
           mbar_wait(&ms.slot_free[prev2.slot], prev2.phase, wt, kSitePv, kb);
           __syncwarp();
         }
-        if (live) {
+        auto put_p = [&]() -> float {
+          float sum = 0.f;
           const uint32_t rope = sbase + PL::kOffKV + at.slot * kSlot + (kChunks - 1) * kChunk;
-          const uint32_t ph = h == 0 ? rope : R == 64 ? sbase + PL::kOffP + (kb & 1) * PL::kPHalf : rope + PL::kPHalf;
+          const uint32_t ph = h == 0 ? rope : sbase + PL::kOffP + (kb & 1) * PL::kPHalf;
           // 8 rows x 8 keys a matrix of 128 bytes: rows first, then keys
-          const uint32_t to = ph + 2 * c * (R * 16) + r * 16;
-          uint32_t u[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = fast_exp2(v[2 * e] - m), b = fast_exp2(v[2 * e + 1] - m);
-            l += a + b;
-            u[e] = bf16x2(a, b);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float a = fast_exp2(v[8 * j + 2 * e] - m), b = fast_exp2(v[8 * j + 2 * e + 1] - m);
+              sum += a + b;
+              u[e] = bf16x2(a, b);
+            }
+            st_shared16(ph + j * (R * 16) + r * 16, make_uint4(u[0], u[1], u[2], u[3]));
           }
-          st_shared16(to, make_uint4(u[0], u[1], u[2], u[3]));
-          st_shared16(to + R * 16, make_uint4(u[4], u[5], u[6], u[7]));
+          fence_proxy_async_smem();
+          tc_fence_before();
+          return sum;
+        };
+        // P is written as if no row needed a new maximum
+        float sum = need ? 0.f : put_p();
+        bool change = group_any(c, need);
+        if (!first) {
+          mbar_wait(&ms.decided, (kb - 1) & 1, wt, kSiteVote, kb);
+          __syncwarp();
+          if (renew()) {                                    // (all four warps)
+            change = group_any(c, must());
+            if (!change) {
+              sum = put_p();
+              group_any(c, false);
+            }
+          }
         }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(a_p_ready + 8u * at.slot);
-        prev2 = prev; prev = at; at.advance();
+        if (change) {
+          ms.top[h][r] = mx;
+          group_any(c, false);
+          const float now = fmaxf(m, fmaxf(ms.top[0][r], ms.top[1][r])), f = fast_exp2(m - now);
+          m = now;
+          l *= f;
+          if (h == 0) {
+            ms.most[r] = m;
+            if (!first) {
+              ms.corr[r] = f;
+              st_cluster_f32(mapa(smem_u32(&ms.corr_peer[r]), peer), f);
+            }
+          }
+          if (!first) {
+            // the columns of these rows: this CTA's dims here, the peer's by its four warps
+            const uint32_t asked = *asks;
+            fence_cluster();
+            group_any(c, false);
+            if ((threadIdx.x & 127) == 0) {
+              st_cluster_u32(mapa(smem_u32(&ms.asked_slot), peer), (uint32_t)prev.slot);
+              st_cluster_u32(mapa(smem_u32(&ms.asked_phase), peer), prev.phase);
+              mbar_arrive_cluster_release(mapa(smem_u32(&ms.asked), peer));
+            }
+            mbar_wait(&ms.slot_free[prev.slot], prev.phase, wt, kSitePv, kb);
+            __syncwarp();
+            for (int i = 0; i < 2; ++i) rescale(tmem + lane_base + kTile * i + R * cta, ms.corr);
+            wait_cluster(&ms.answered, asked & 1, wt, kSiteAid, kb);
+            __syncwarp();
+            if ((threadIdx.x & 127) == 0) *asks = asked + 1;
+          }
+          sum = put_p();
+          ++seen;
+          group_any(c, false);
+          if ((threadIdx.x & 127) == 0) *changes = seen;
+        }
+        l += sum;
+        if ((threadIdx.x & 127) == 0) {                     // (all warps have fenced what they wrote)
+          mbar_arrive(&ms.decided);
+          mbar_arrive_cluster(a_p_ready + 8u * at.slot);
+        }
       }
+      softmax_sync();                                       // (after the last block's change)
+      renew();
       // epilogue: this CTA's dims of all of the tile's rows
-      softmax_sync();                                       // (the maxima have been read)
-      if (live) ms.top[2 * c + h][r] = l;
+      ms.top[2 * c + h][r] = l;
       const bool whole = w.whole();
       const int slot = cluster * 2 + (w.index == 0 ? 0 : 1);
       softmax_sync();
-      if (live && h == 0 && c == 0) {
+      if (h == 0 && c == 0) {
         const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r], f = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
         ms.scale[R * cta + r] = f;
         st_cluster_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f);
@@ -305,13 +371,17 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
           tmem_wait_ld();
           if (x + 16 < kTile) tmem_ld16(tmem + lane_base + kTile * c + x + 16, o[y ^ 1]);
           if (whole) {
-            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kTile + x) * kDV + d;
+            // Lanes 2 i and 2 i + 1 exchange, for two dims of a row each
+            const int odd = lane & 1;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out) + (((long long)w.b * p.rows + rt * kTile + x + odd) * kDV + (d & ~1)) / 2;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (x + e < rows) {
-                const float f = ms.scale[x + e];
-                dst[e * kDV] = __float2bfloat16(f > 0.f ? o[y][e] * f : 0.f);      // a row without keys: 0, whatever the values of others
+            for (int e = 0; e < 16; e += 2) {
+              const float got = __shfl_xor_sync(0xffffffffu, odd ? o[y][e] : o[y][e + 1], 1), a = odd ? got : o[y][e], b = odd ? o[y][e + 1] : got;
+              if (x + e + odd < rows) {
+                const float f = ms.scale[x + e + odd];
+                dst[e * (kDV / 2)] = f > 0.f ? bf16x2(a * f, b * f) : 0u;          // a row without keys: 0, whatever the values of others
               }
+            }
           } else {
             float* dst = p.part_o + ((long long)slot * kTile + x) * kDV + d;
 #pragma unroll
@@ -321,7 +391,28 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         }
       }
       tc_fence_before();
+      softmax_sync();                                       // (either group's P may start the next piece)
       more = w.next(p);
+    }
+    // The peer asks for nothing any more: all of its P are in O.
+    if (threadIdx.x == 0) {
+      *reinterpret_cast<volatile uint32_t*>(&ms.over) = 1;
+      mbar_arrive(&ms.asked);
+    }
+  } else if (warp >= kWarpAid<kLoad>) {
+    // ------------------------------------------------------------ rescalings that the peer asks for
+    const int quarter = warp & 3;
+    const uint32_t a_answered = mapa(smem_u32(&ms.answered), peer);
+    for (uint32_t n = 0;; ++n) {
+      // (Most launches ask for none, so this wait may last as long as the launch; it ends with the softmax warps, whose waits are bounded.)
+      uint32_t ok = 0;
+      for (uint32_t i = 0; !ok && !wt.aborting() && i < (1u << 24); ++i) ok = try_wait_cluster(&ms.asked, n & 1);
+      if (aid_any(!ok || *reinterpret_cast<volatile uint32_t*>(&ms.over) != 0)) break;      // (all four warps or none)
+      const uint32_t slot = *reinterpret_cast<volatile uint32_t*>(&ms.asked_slot), phase = *reinterpret_cast<volatile uint32_t*>(&ms.asked_phase);
+      mbar_wait(&ms.slot_free[slot < kSlots ? slot : 0], phase, wt, kSiteAid, (int)n);
+      __syncwarp();
+      for (int c = 0; c < 2; ++c) rescale(tmem + ((uint32_t)(32 * quarter) << 16) + kTile * c + R * peer, ms.corr_peer);
+      if (!aid_any(false) && warp == kWarpAid<kLoad> && lane == 0) mbar_arrive_cluster_release(a_answered);
     }
   } else if (warp == kWarpQk) {
     // ------------------------------------------------------------ S = Q K^T (the leader, one thread)
@@ -377,7 +468,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
           const uint32_t slot = sbase + PL::kOffKV + at.slot * kSlot, rope = slot + (kChunks - 1) * kChunk;
           const uint64_t vd = umma_desc(slot, kChunk, 1024, kSwz128);               // dims along M: two chunks of 64, 8 keys 1024 bytes
           const uint64_t pd = umma_desc(rope, R * 16, 128, kSwzNone);
-          const uint32_t p1 = R == 64 ? sbase + PL::kOffP + (kb & 1) * PL::kPHalf : rope + PL::kPHalf;
+          const uint32_t p1 = sbase + PL::kOffP + (kb & 1) * PL::kPHalf;
           const uint32_t v_lo = (uint32_t)vd, v_hi = (uint32_t)(vd >> 32), p_hi = (uint32_t)(pd >> 32), p1_lo = (uint32_t)umma_desc(p1, R * 16, 128, kSwzNone);
 #pragma unroll 1
           for (int i = 0; i < 2; ++i) {
@@ -418,109 +509,133 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         cp_async_wait_all();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(a_ready);
+        if (lane == 0) mbar_arrive_cluster(a_ready);
       }
       ++asked;
     }
     if (!ok && asked > 0 && lane == 0 && cta == 0) mbar_drain(&ms.q_ready, (asked - 1) & 1);        // given up: what is in flight lands first
     __syncwarp();
-  } else if (kLoad == kTma ? warp <= kWarpV : warp >= kLoad0) {
+  } else if (kLoad == kPacked && warp == kWarpBring) {
+    // ------------------------------------------------------------ this CTA's keys into L2, two blocks ahead of the converting warps
+    const int count = ms.count;
+    Ahead<true> next(ms, p, kOwnKeys * (int)cta, kOwnKeys, lane);
+    Turn mine_to_bring{p.row_tiles, rt};
+    Cursor at;
+    for (int kb = 0; kb < count; ++kb, next.advance(p, lane)) {
+      if (kb >= kSlots) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&ms.slot_free[at.slot], at.phase ^ 1u, wt, kSiteFree, kb))) break;
+      }
+      at.advance();
+      if (!mine_to_bring()) continue;
+      for (int d = kb == 0 ? 0 : 2; d < 3; ++d) {
+        const int n = next.rows_in(d), row = __shfl_sync(0xffffffffu, next.row, next.i + d), one = min(n, p.block_size - row);
+        const uint8_t* src = next.rows_of(p, d, kPackedRow);
+        if (src != nullptr && lane == 0 && one > 0) l2_prefetch_1d(src, (uint32_t)(one * kPackedRow));
+        const int page2 = __shfl_sync(0xffffffffu, next.page2, next.i + d);
+        if (one < n && page2 < p.n_blocks && lane == 0) l2_prefetch_1d(p.cache + (long long)page2 * p.block_pitch, (uint32_t)((n - one) * kPackedRow));
+      }
+    }
+  } else if (kLoad == kTma ? warp <= kWarpK1 : warp >= kLoad0) {
     // ------------------------------------------------------------ keys (own 32, all dims) and values (the peer's 32, own 256 dims)
-    // kTma: a warp each, chunks of 32 rows of a page.  Else a warp has some adjacent rows (of a page: pages are multiples of 16 rows).
-    constexpr int kHalfWarps = kLoad == kTma ? 1 : kLoaders<kLoad> / 2, kRowsOwn = kOwnKeys / kHalfWarps;
     constexpr int kRowBytes = kLoad == kPacked ? kPackedRow : 2 * kD;
-    const bool is_v = kLoad == kTma ? warp == kWarpV : warp - kLoad0 >= kHalfWarps;
-    const int part = kLoad == kTma ? 0 : (warp - kLoad0) % kHalfWarps, first_row = kRowsOwn * part;      // of the 32
+    const bool is_v = kLoad == kTma ? warp == kWarpV : warp >= kLoad0 + kKeyWarps;
+    // The warp's rows of the 32.  kTma: pages of multiples of 32 rows have one box of rows a chunk, others two; keys of one box are shared out by chunks, of
+    // two by box.  kPacked: 4 rows a warp of keys, 8 of values (of one page: pages are multiples of 16 rows).
+    const int boxes = kLoad == kTma ? kOwnKeys / p.box_rows : 1, second = kLoad == kTma && warp == kWarpK1 ? 1 : 0;
+    const int rows_own = kLoad == kTma ? (is_v || boxes == 1 ? kOwnKeys : 16) : is_v ? kOwnKeys / kValueWarps : kOwnKeys / kKeyWarps;
+    const int first_row = kLoad == kTma ? (rows_own < kOwnKeys ? 16 * second : 0) : rows_own * (is_v ? warp - kLoad0 - kKeyWarps : warp - kLoad0);
+    const int box = kLoad == kTma && is_v && boxes > 1 ? (lane >> 2) & 1 : 0;        // the lane's, for values
     const int half = is_v ? (int)peer : (int)cta;                                    // whose keys
     const uint32_t a_full = mapa(smem_u32(is_v ? &ms.v_full[0] : &ms.k_full[0]), 0);
     uint64_t* const waits = is_v ? ms.qk_done : ms.slot_free;
     const uint32_t chunk0 = is_v ? (cta == 0 ? 4 : 0) : 0;                           // where its first chunk goes
     const int dim0 = is_v ? 256 * (int)cta : 0;
-    struct Coming { int page, row, n; };                                             // n of the warp's rows hold keys
-    Walk w(ms);
     const int count = ms.count;
-    int k_at = 0, looked = 0;
-    if (w.next(p)) k_at = w.k0;
-    auto look = [&]() -> Coming {
-      Coming x{-1, 0, 0};
-      if (looked >= count) return x;
-      const int key = k_at * kBlock + kOwnKeys * half + first_row;
-      x.n = min(max(w.len - key, 0), kRowsOwn);
-      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + key / p.block_size);
-      x.row = key % p.block_size;
-      ++looked;
-      if (++k_at == w.k1 && w.next(p)) k_at = w.k0;
-      return x;
-    };
-    auto rows_of = [&](const Coming& x) -> const uint8_t* {
-      return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kRowBytes : nullptr;
-    };
-    auto to_l2 = [&](const Coming& x) {                     // (the other rows are the peer's to bring in)
-      const uint8_t* src = rows_of(x);
-      if (!is_v && src != nullptr && lane == 0) l2_prefetch_1d(src, (uint32_t)(x.n * kRowBytes));
-    };
     // a slot is free (K) or its keys have been read (V)
     auto free_for = [&](const Cursor& at, int kb) -> bool {
       if (is_v) return mbar_wait(&waits[at.slot], at.phase, wt, kSiteFree, kb);
       return kb < kSlots || mbar_wait(&waits[at.slot], at.phase ^ 1u, wt, kSiteFree, kb);
     };
-    // 16-byte pieces of rows first_row .. + kRowsOwn, zeros behind the keys
-    auto copy_rows = [&](const Coming& x, uint32_t slot) {
-      const uint8_t* src = rows_of(x);
-      const int pieces = is_v ? 32 : kD / 8;
-      for (int y = lane; y < kRowsOwn * pieces; y += 32) {
-        const int r = y / pieces, c = y - r * pieces, row = first_row + r;
-        const bool in = src != nullptr && r < x.n;
-        cp_async16_or_zero(slot + (chunk0 + (c >> 3)) * kChunk + row * 128 + (((c & 7) ^ (row & 7)) << 4), in ? src + (long long)r * kRowBytes + 2 * dim0 + 16 * c : p.cache, in);
-      }
-    };
     Cursor at;
     bool ok = true;
-    Coming c0 = look(), c1 = look(), c2 = look();
+    // The page, row and number of the warp's rows of a block, for the loads through registers
+    struct Coming { int page, row, n; };
+    Walk w(ms);
+    int k_at = 0, looked = 0;
+    PageAt pa(p.block_size);
+    auto piece = [&]() {
+      if (!w.next(p)) return;
+      k_at = w.k0;
+      pa.at(k_at * kBlock + kOwnKeys * half + first_row);
+    };
+    auto look = [&]() -> Coming {
+      Coming x{-1, 0, 0};
+      if (looked >= count) return x;
+      x.n = min(max(w.len - k_at * kBlock - kOwnKeys * half - first_row, 0), rows_own);
+      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + pa.page);
+      x.row = pa.row;
+      ++looked;
+      pa.advance();
+      if (++k_at == w.k1) piece();
+      return x;
+    };
+    auto rows_of = [&](const Coming& x) -> const uint8_t* {
+      return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kRowBytes : nullptr;
+    };
+    if (kLoad == kPacked) piece();
     if (kLoad != kPacked) {
-      const uint64_t pol = l2_policy_evict_first();
-      int asked = 0, pending = -1;                          // slot whose copies are under way (kCopy)
-      auto announce = [&]() {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(a_full + 8u * pending);
-        pending = -1;
+      Ahead<true> next(ms, p, kOwnKeys * half + first_row, rows_own, lane);
+      Turn mine_to_bring{p.row_tiles, rt};
+      // (the other rows are the peer's to bring in)
+      auto to_l2 = [&](int d) {
+        const uint8_t* src = next.rows_of(p, d, kRowBytes);
+        const int n = next.rows_in(d);
+        if (!is_v && src != nullptr && lane == 0 && (rows_own < kOwnKeys || second == 0)) l2_prefetch_1d(src, (uint32_t)(n * kRowBytes));
       };
-      if (kLoad == kCopy) { to_l2(c0); to_l2(c1); }
-      for (int kb = 0; kb < count; ++kb) {
-        const Coming c3 = look();
+      const uint64_t pol = l2_policy_evict_first();
+      int asked = 0;
+      // what the lane requests of a block
+      const int chunk = is_v ? lane & 3 : boxes == 1 ? lane + 5 * second : lane;
+      const bool mine = is_v ? lane < 4 * boxes : boxes == 1 ? (second ? lane < 4 : lane < 5) : lane < kChunks;
+      const uint32_t bytes = (is_v ? 4u * kChunk : boxes == 1 ? (second ? 4u : 5u) * kChunk : kChunks * kChunk / 2);
+      for (int kb = 0; kb < count; ++kb, next.advance(p, lane)) {
         const uint32_t slot = sbase + PL::kOffKV + at.slot * kSlot;
-        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
-        // a block's copies land while the next one's are issued, unless there is nothing to issue yet
-        const bool idle = is_v ? !mbar_test(&waits[at.slot], at.phase) : kb >= kSlots && !mbar_test(&waits[at.slot], at.phase ^ 1u);
-        if (pending >= 0 && __any_sync(0xffffffffu, idle)) { cp_async_wait_all(); announce(); }
+        const int n = next.rows_in(0), page1 = __shfl_sync(0xffffffffu, next.page, next.i), page2 = __shfl_sync(0xffffffffu, next.page2, next.i);
+        const int row1 = __shfl_sync(0xffffffffu, next.row, next.i), row2 = row1 + 16 - (row1 + 16 >= p.block_size ? p.block_size : 0);
+        if (mine_to_bring()) to_l2(2);
         if (!(ok = __all_sync(0xffffffffu, free_for(at, kb)))) break;
-        const int chunks = is_v ? 4 : kChunks;
-        if (kLoad == kTma && c0.n == kOwnKeys) {
-          if (lane == 0) arrive_expect_cluster(a_full + 8u * at.slot, chunks * kChunk);
+        if (n == rows_own || n == 0) {                      // (of a page beyond the cache, or none: zeros)
+          if (lane == 0) arrive_expect_cluster(a_full + 8u * at.slot, bytes);
           __syncwarp();
-          if (lane < chunks)
-            tma_load_3d_pair_hint(slot + (chunk0 + lane) * kChunk, &map_kv, dim0 + 64 * lane, c0.row, (unsigned)c0.page < (unsigned)p.n_blocks ? c0.page : p.n_blocks,
-                                  a_full + 8u * at.slot, pol);
+          if (mine)
+            tma_load_3d_pair_hint(slot + (chunk0 + chunk) * kChunk + (first_row + 16 * box) * 128, &map_kv, dim0 + 64 * chunk, box ? row2 : row1,
+                                  box ? page2 : page1, a_full + 8u * at.slot, pol);
           asked = kb + 1;
         } else {
-          copy_rows(c0, slot);                              // (kTma: the rows at a sequence's end, and none)
-          cp_async_commit();
-          if (pending >= 0) { cp_async_wait_but_one(); announce(); }
-          pending = at.slot;
-          if (kLoad == kTma) { cp_async_wait_all(); announce(); }
+          // zeros behind a sequence's end: 0 x NaN is NaN
+          for (int x = second == 0 || boxes > 1 ? 0 : rows_own; x < rows_own; x += 16) {
+            const int page = x ? page2 : page1, rows = page < p.n_blocks ? n - x : 0;
+            const uint8_t* from = p.cache + (page < p.n_blocks ? (long long)page * p.block_pitch + (long long)(x ? row2 : row1) * kRowBytes + 2 * dim0 + 16 * lane : 0);
+            const uint32_t to = slot + (chunk0 + (lane >> 3)) * kChunk + (first_row + x) * 128;
+            for (int c = 0; c < (is_v ? 1 : 3); ++c)        // 512 bytes of each row
+              if (c < 2 || lane < 8)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  cp_async16_or_zero(to + 4 * c * kChunk + r * 128 + (((lane & 7) ^ (r & 7)) << 4), r < rows ? from + 512 * c + r * kRowBytes : p.cache, r < rows);
+          }
+          cp_async_wait_all();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(a_full + 8u * at.slot);
         }
         at.advance();
-        c0 = c1; c1 = c2; c2 = c3;
       }
-      cp_async_wait_all();
-      if (pending >= 0) announce();
       if (!ok && asked > 0) __nanosleep(100000);            // given up: what is in flight lands first (some microseconds; its barrier is the leader's)
     } else if (!is_v) {
       // Of each 128 dims eight lanes have 16 codes of a row each, four rows at a time.  A group's registers are loaded for the next
       // block as soon as they are converted for this one, from L2, where the rows were brought a block before.
       const int sub = lane >> 3, c = lane & 7, row = first_row + sub;
-      static_assert(kLoad != kPacked || kRowsOwn == 4, "a row a lane group");
+      static_assert(kOwnKeys / kKeyWarps == 4 && kOwnKeys / kValueWarps == 8, "rows of a warp");
       uint4 codes[4], rope;
       float4 scale;
       const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -532,13 +647,11 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         for (int j = 0; j < 4; ++j) codes[j] = in ? __ldcg(reinterpret_cast<const uint4*>(from + 128 * j) + c) : zero;
         rope = in ? __ldcg(reinterpret_cast<const uint4*>(from + 528) + c) : zero;
       };
-      to_l2(c0);
-      to_l2(c1);
-      load(rows_of(c0), c0.n);
+      Coming c1 = look(), c2 = look();
+      load(rows_of(c1), c1.n);
       for (int kb = 0; ok && kb < count; ++kb) {
-        const Coming c3 = look();
+        c1 = c2; c2 = look();                               // (moved before the next is asked for: a move waits for its load)
         const uint32_t slot = sbase + PL::kOffKV + at.slot * kSlot;
-        if ((looked + rt) % p.row_tiles == 0) to_l2(c2);
         if (!(ok = __all_sync(0xffffffffu, free_for(at, kb)))) break;
         const float f[4] = {scale.x, scale.y, scale.z, scale.w};
 #pragma unroll
@@ -553,33 +666,33 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         st_shared16(slot + (kChunks - 1) * kChunk + row * 128 + ((c ^ (row & 7)) << 4), rope);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(a_full + 8u * at.slot);
-        load(rows_of(c1), c1.n);
+        if (lane == 0) mbar_arrive_cluster(a_full + 8u * at.slot);
+        load(rows_of(c1), c1.n);                            // (the next)
         at.advance();
-        c0 = c1; c1 = c2; c2 = c3;
       }
     } else {
       // the peer's rows: 16 lanes a row, 16 codes each of this CTA's 256 dims
       const int sub = lane >> 4, c = lane & 15;
-      uint4 codes[2];
-      float scale[2];
+      uint4 codes[4];
+      float scale[4];
       const uint4 zero = make_uint4(0, 0, 0, 0);
       auto load = [&](const uint8_t* src, int n) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const bool in = src != nullptr && sub + 2 * i < n;
           const uint8_t* from = src + (sub + 2 * i) * kRowBytes;
           codes[i] = in ? __ldcg(reinterpret_cast<const uint4*>(from + dim0) + c) : zero;
           scale[i] = in ? __ldcg(reinterpret_cast<const float*>(from + 512) + dim0 / 128 + (c >> 3)) : 0.f;
         }
       };
-      load(rows_of(c0), c0.n);
+      Coming c1 = look(), c2 = look();
+      load(rows_of(c1), c1.n);
       for (int kb = 0; ok && kb < count; ++kb) {
-        const Coming c3 = look();
+        c1 = c2; c2 = look();                               // (moved before the next is asked for: a move waits for its load)
         const uint32_t slot = sbase + PL::kOffKV + at.slot * kSlot;
         if (!(ok = __all_sync(0xffffffffu, free_for(at, kb)))) break;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int row = first_row + sub + 2 * i;
           uint4 a, b;
           convert16(codes[i], scale[i], a, b);
@@ -589,10 +702,9 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_release(a_full + 8u * at.slot);
-        load(rows_of(c1), c1.n);
+        if (lane == 0) mbar_arrive_cluster(a_full + 8u * at.slot);
+        load(rows_of(c1), c1.n);                            // (the next)
         at.advance();
-        c0 = c1; c1 = c2; c2 = c3;
       }
     }
   }
@@ -610,33 +722,32 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
 }
 
 // pairs that can run at once
-template <int R, Load kLoad>
+template <Load kLoad>
 static int pairs() {
   static thread_local int cached_dev = -1, cached = 0;
   const int dev = current_device();
   if (dev == cached_dev) return cached;
   int n = sm_count() / 2, q = 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sm_count()); cfg.blockDim = dim3(kPairThreads<kLoad>); cfg.dynamicSmemBytes = PairPlan<R>::kSmem;
+  cfg.gridDim = dim3((unsigned)sm_count()); cfg.blockDim = dim3(kPairThreads<kLoad>); cfg.dynamicSmemBytes = PL::kSmem;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
   cfg.attrs = &at; cfg.numAttrs = 1;
-  if (ensure_smem<mla_decode_pair_kernel<R, kLoad>>(dev, PairPlan<R>::kSmem) &&
-      cudaOccupancyMaxActiveClusters(&q, mla_decode_pair_kernel<R, kLoad>, &cfg) == cudaSuccess && q > 0)
+  if (ensure_smem<mla_decode_pair_kernel<kLoad>>(dev, PL::kSmem) &&
+      cudaOccupancyMaxActiveClusters(&q, mla_decode_pair_kernel<kLoad>, &cfg) == cudaSuccess && q > 0)
     n = q;
   cudaGetLastError();
   cached_dev = dev; cached = n;
   return n;
 }
-template <int R, Load kLoad>
+template <Load kLoad>
 static int launch(const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
-  if (!ensure_smem<mla_decode_pair_kernel<R, kLoad>>(current_device(), PairPlan<R>::kSmem)) return LITEDSA_ERR_CUDA;
-  return launch_pdl(mla_decode_pair_kernel<R, kLoad>, dim3((unsigned)(2 * p.groups * p.row_tiles)), kPairThreads<kLoad>, PairPlan<R>::kSmem, st, map, map_q, p);
+  if (!ensure_smem<mla_decode_pair_kernel<kLoad>>(current_device(), PL::kSmem)) return LITEDSA_ERR_CUDA;
+  return launch_pdl(mla_decode_pair_kernel<kLoad>, dim3((unsigned)(2 * p.groups * p.row_tiles)), kPairThreads<kLoad>, PL::kSmem, st, map, map_q, p);
 }
-template <int R>
 static int launch(Load l, const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
-  return l == kTma ? pair::launch<R, kTma>(map, map_q, p, st) : l == kCopy ? pair::launch<R, kCopy>(map, map_q, p, st) : pair::launch<R, kPacked>(map, map_q, p, st);
+  return l == kTma ? pair::launch<kTma>(map, map_q, p, st) : pair::launch<kPacked>(map, map_q, p, st);
 }
 
 }  // namespace pair
