@@ -204,6 +204,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------------ softmax, epilogue
+    if (kLoad == kPacked) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");     // 2 x 88 + 4 x 72 + 40 = 7 x 72, as launched
     // Two groups of four warps take turns, a block each: warp (warp % 4) has TMEM lanes 32 (warp % 4), a thread row r and keys 32 h + [0, 32).
     // Blocks' maxima are settled in order (decided): whoever finds a row past its bound changes the row's for both groups, which
     // the other sees before it hands its P over.
@@ -215,7 +216,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
     Walk w(ms);
     Cursor at, prev, prev2;                                 // of blocks kb, kb - 1, kb - 2
     int kb = 0;
-    uint32_t seen = 0;                                      // changes
+    uint32_t seen = 0, wholes = 0;                          // changes; sequences ended here
     // A wait here that gives up is passed like any other: the warps meet at named barriers, so they take the same steps.
     bool more = w.next(p);
     while (more) {
@@ -344,19 +345,22 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
       const int slot = cluster * 2 + (w.index == 0 ? 0 : 1);
       softmax_sync();
       if (h == 0 && c == 0) {
-        const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r], f = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
-        ms.scale[R * cta + r] = f;
-        st_cluster_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f);
+        const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r];
         if (whole) {
+          const float f = sum > 0.f ? 1.f / sum : 0.f;
+          ms.scale[R * cta + r] = f;
+          st_cluster_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f);
           if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m + __log2f(sum)) * kLn2 : INFINITY;
         } else {
           p.part_ml[(long long)slot * kTile + R * cta + r] = make_float2(m, sum);
         }
       }
-      fence_cluster();
-      softmax_sync();
-      if (threadIdx.x == 0) mbar_arrive_cluster_release(mapa(smem_u32(&ms.fin_full), peer));
-      wait_cluster(&ms.fin_full, w.index & 1, wt, kSiteVote, kb);
+      if (whole) {                                          // (both CTAs alike)
+        fence_cluster();
+        softmax_sync();
+        if (threadIdx.x == 0) mbar_arrive_cluster_release(mapa(smem_u32(&ms.fin_full), peer));
+        wait_cluster(&ms.fin_full, wholes++ & 1, wt, kSiteVote, kb);
+      }
       mbar_wait(&ms.slot_free[prev.slot], prev.phase, wt, kSitePv, kb);
       __syncwarp();
       tc_fence_after();
@@ -401,6 +405,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
     }
   } else if (warp >= kWarpAid<kLoad>) {
     // ------------------------------------------------------------ rescalings that the peer asks for
+    if (kLoad == kPacked) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     const int quarter = warp & 3;
     const uint32_t a_answered = mapa(smem_u32(&ms.answered), peer);
     for (uint32_t n = 0;; ++n) {
@@ -563,16 +568,18 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
     Walk w(ms);
     int k_at = 0, looked = 0;
     PageAt pa(p.block_size);
+    const int* table = nullptr;
     auto piece = [&]() {
       if (!w.next(p)) return;
       k_at = w.k0;
+      table = p.table + w.b * p.table_pitch;
       pa.at(k_at * kBlock + kOwnKeys * half + first_row);
     };
     auto look = [&]() -> Coming {
       Coming x{-1, 0, 0};
       if (looked >= count) return x;
       x.n = min(max(w.len - k_at * kBlock - kOwnKeys * half - first_row, 0), rows_own);
-      if (x.n > 0) x.page = __ldcg(p.table + w.b * p.table_pitch + pa.page);
+      if (x.n > 0) x.page = __ldcg(table + pa.page);
       x.row = pa.row;
       ++looked;
       pa.advance();
