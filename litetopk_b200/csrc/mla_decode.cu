@@ -283,8 +283,9 @@ __device__ __forceinline__ void convert16(const uint4& c, float scale, uint4& a,
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> (16 * k)), __NV_E4M3);
-      const float2 f = __half22float2(__half2(h));
-      o[2 * i + k] = bf16x2(f.x * scale, f.y * scale);
+      float2 f = __half22float2(__half2(h));
+      asm("{\n\t.reg .b64 x, s;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmul.rn.f32x2 x, x, s;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+f"(f.x), "+f"(f.y) : "f"(scale));
+      o[2 * i + k] = bf16x2(f.x, f.y);
     }
   }
   a = make_uint4(o[0], o[1], o[2], o[3]);
