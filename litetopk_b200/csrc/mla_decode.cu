@@ -787,56 +787,107 @@ __device__ __forceinline__ void add_parts(const Params& p, int kRows, int g, con
     }
   }
 }
-__global__ void __launch_bounds__(32 * kMergeWarps, 3) mla_decode_merge_kernel(const Params p, int kRows) {
+// Up to 8 parts: the first three are asked for before their weights are known.
+__device__ __forceinline__ void add_few(const Params& p, int kRows, int g, const int4& e, int row, float4 (&a)[4], float& l, float& m, int lane) {
+  const int rt = row / kRows, r = row - rt * kRows;
+  const long long s0 = ((long long)(g * p.row_tiles + rt) * 2 + e.y) * kRows + r, ds = 2LL * p.row_tiles * kRows, s1 = s0 - (long long)e.y * kRows;
+  auto slot = [&](int i) { return i == 0 ? s0 : s1 + i * ds; };
+  float4 v[3][4];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (i0 + u < e.z) {
+        const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(i0 + u) * kDV);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[u][c] = __ldcg(src + 32 * c + lane);
+      }
+  };
+  float2 ml = make_float2(kMInit, 0.f);
+  if (lane < e.z) ml = __ldcg(&p.part_ml[slot(lane)]);
+  load(0);
+  m = ml.x;
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  m = __shfl_sync(0xffffffffu, m, 0);
+  const float w = fast_exp2(ml.x - m);
+#pragma unroll
+  for (int i0 = 0; i0 < 8; i0 += 3) {
+    if (i0 >= e.z) break;
+    if (i0) load(i0);
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      const float f = __shfl_sync(0xffffffffu, w, i0 + u), y = __shfl_sync(0xffffffffu, ml.y, i0 + u);
+      if (!(y > 0.f)) continue;                        // beyond the list, or a part without keys
+      l += f * y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        a[c].x += f * v[u][c].x; a[c].y += f * v[u][c].y; a[c].z += f * v[u][c].z; a[c].w += f * v[u][c].w;
+      }
+    }
+  }
+}
+__global__ void __launch_bounds__(32 * kMergeWarps, 2) mla_decode_merge_kernel(const Params p, int kRows) {
   __shared__ float4 acc[kMergeWarps][kDV / 4];
   __shared__ float sum_l[kMergeWarps];
-  __shared__ int list[kMaxGroups], units[kMaxGroups + 1], n_list;
+  __shared__ int4 list[kMaxGroups];                    // {sequence, slot of its first part, parts, group of the first}
+  __shared__ int units[kMaxGroups + 1], found[2][kMergeWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_trigger();
   pdl_wait();
-  if (warp == 0) {                                     // the cut sequences, and where each one's units of work begin
-    int n = 0, u = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-      const int parts = g0 + lane < p.groups && __ldcg(&p.meta[g0 + lane].x) >= 0 ? __ldcg(&p.meta[g0 + lane].z) : 0;
-      const uint32_t mask = __ballot_sync(0xffffffffu, parts > 0);
-      const int mine = parts == 0 ? 0 : parts <= 8 ? (p.rows + kMergeWarps - 1) / kMergeWarps : p.rows;
-      int incl = mine;
+  // The cut sequences, and where each one's units of work begin
+  int n = 0, all = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += 32 * kMergeWarps) {
+    const int g = g0 + (int)threadIdx.x;
+    int4 e = make_int4(-1, 0, 0, 0);
+    if (g < p.groups) e = __ldcg(p.meta + g);
+    const bool cut = e.x >= 0 && e.z > 0;
+    const int mine = !cut ? 0 : e.z <= 8 ? (p.rows + kMergeWarps - 1) / kMergeWarps : p.rows;
+    const uint32_t mask = __ballot_sync(0xffffffffu, cut);
+    int incl = mine;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
-      }
-      if (parts > 0) {
-        const int at = n + __popc(mask & ((1u << lane) - 1u));
-        list[at] = g0 + lane;
-        units[at] = u + incl - mine;
-      }
-      n += __popc(mask);
-      u += __shfl_sync(0xffffffffu, incl, 31);
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
     }
-    if (lane == 0) { units[n] = u; n_list = n; }
+    if (lane == 31) { found[0][warp] = __popc(mask); found[1][warp] = incl; }
+    __syncthreads();
+    int at = n + __popc(mask & ((1u << lane) - 1u)), before = all + incl - mine;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+      if (w < warp) { at += found[0][w]; before += found[1][w]; }
+      n += found[0][w];
+      all += found[1][w];
+    }
+    if (cut) {
+      list[at] = make_int4(e.x, e.y, e.z, g);
+      units[at] = before;
+    }
+    __syncthreads();
   }
+  if (threadIdx.x == 0) units[n] = all;
   __syncthreads();
-  const int n = n_list, all = units[n];
   int at = 0;
   for (int u = (int)blockIdx.x; u < all; u += (int)gridDim.x) {
     while (units[at + 1] <= u) ++at;
-    const int g = list[at];
-    const int4 e = __ldcg(p.meta + g);
+    const int4 e = list[at];
+    const int g = e.w;
     const bool alone = e.z <= 8;                       // a warp a row
     const int row = alone ? (u - units[at]) * kMergeWarps + warp : u - units[at];
     if (row < p.rows) {                                // (the same for all of a block that shares a row)
-      const int rt = row / kRows, r = row - rt * kRows;
-      float m = kMInit;
-      for (int i = lane; i < e.z; i += 32)
-        m = fmaxf(m, __ldcg(&p.part_ml[((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r].x));
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
       float4 a[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
-      add_parts(p, kRows, g, e, row, m, alone ? 0 : warp, alone ? 1 : kMergeWarps, a, l, lane);
+      float l = 0.f, m = kMInit;
+      if (alone) {
+        add_few(p, kRows, g, e, row, a, l, m, lane);
+      } else {
+        const int rt = row / kRows, r = row - rt * kRows;
+        for (int i = lane; i < e.z; i += 32)
+          m = fmaxf(m, __ldcg(&p.part_ml[((long long)((g + i) * p.row_tiles + rt) * 2 + (i == 0 ? e.y : 0)) * kRows + r].x));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        add_parts(p, kRows, g, e, row, m, warp, kMergeWarps, a, l, lane);
+      }
       const long long to = (long long)e.x * p.rows + row;
       if (alone) {
         const float f = l > 0.f ? 1.f / l : 0.f;
@@ -966,7 +1017,7 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
                  : s.per == 64 ? launch<64>(load, map, map_q, p, st) : pair::launch(load, map, map_q, p, st);
   if (rc != LITEDSA_OK || s.groups == 1) return rc;
   const int64_t most = (int64_t)min(B, s.groups) * p.rows;                 // rows that can need it
-  return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)min(most, (int64_t)3 * sm_count())), 32 * kMergeWarps, 0, st, p, s.per);
+  return launch_pdl(mla_decode_merge_kernel, dim3((unsigned)min(most, (int64_t)2 * sm_count())), 32 * kMergeWarps, 0, st, p, s.per);
 }
 
 // Status block of the kernel; layout and return rule as litedsa_attn_status.
