@@ -344,6 +344,9 @@ PyObject* mla_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto per_head = [&](const Tensor& t, int64_t rows, int64_t d) {
       return t.dim() == 3 && t.scalar_type() == at::kBFloat16 && t.size(0) == rows && t.size(1) == heads && t.size(2) == d && t.stride(2) == 1;
     };
+    for (const Tensor* t : {q, kn, kr, v})
+      for (int64_t i = 0; i < t->dim(); ++i)
+        if (t->stride(i) == 0) Py_RETURN_NONE;
     if (Tq <= 0 || Tk <= 0 || heads <= 0 || !small(Tq) || !small(Tk) || !small(heads) || !per_head(*q, Tq, 192) || !per_head(*kn, Tk, 128) ||
         !per_head(*v, Tk, 128) || kr->scalar_type() != at::kBFloat16 || kr->size(1) != 64 || kr->stride(1) != 1)
       Py_RETURN_NONE;

@@ -611,7 +611,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         const int row1 = __shfl_sync(0xffffffffu, next.row, next.i), row2 = row1 + 16 - (row1 + 16 >= p.block_size ? p.block_size : 0);
         if (mine_to_bring()) to_l2(2);
         if (!(ok = __all_sync(0xffffffffu, free_for(at, kb)))) break;
-        if (n == rows_own || n == 0) {                      // (of a page beyond the cache, or none: zeros)
+        if (n == rows_own || (n == 0 && p.n_blocks > 0)) {  // (of a page beyond the cache, or none: zeros; a cache without pages has no map)
           if (lane == 0) arrive_expect_cluster(a_full + 8u * at.slot, bytes);
           __syncwarp();
           if (mine)

@@ -668,6 +668,10 @@ extern "C" int litedsa_mla_prefill(const void* q, int64_t q_token_stride, int64_
   if (((uintptr_t)q | (uintptr_t)k_nope | (uintptr_t)k_rope | (uintptr_t)v | (uintptr_t)out | (uintptr_t)workspace) & 15 || ((uintptr_t)lse & 3) ||
       (q_token_stride | q_head_stride | k_token_stride | k_head_stride | k_rope_stride | v_token_stride | v_head_stride) % 8)
     return LITEDSA_ERR_UNSUPPORTED;
+  // (a tensor map has no stride of 0)
+  if ((Tq > 1 && q_token_stride <= 0) || (heads > 1 && q_head_stride <= 0) || (Tk > 1 && (k_token_stride <= 0 || k_rope_stride <= 0 || v_token_stride <= 0)) ||
+      (Tk > 0 && heads > 1 && (k_head_stride <= 0 || v_head_stride <= 0)))
+    return LITEDSA_ERR_UNSUPPORTED;
   if (Tq == 0 || B == 0) return LITEDSA_OK;
   const int64_t tiles = cu_q ? min((int64_t)Tq, Tq / kPair + (int64_t)B) : (Tq + kPair - 1) / kPair;
   Params p = {};

@@ -169,8 +169,8 @@ def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: 
                 out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
     """Expanded latent attention over a batch of sequences: scores ``sm_scale * (q[..., :128] . k_nope + q[..., 128:] . k_rope)``.
 
-    q [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64] (one for all heads), all bf16; any strides that are multiples
-    of 8 with unit inner stride (k_nope and v may be views of one projection).  Sequence b has queries ``cu_seqlens_q[b] : cu_seqlens_q[b + 1]`` and
+    q [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64] (one for all heads), all bf16; any strides but 0 that are multiples
+    of 8, unit inner stride (k_nope and v may be views of one projection).  Sequence b has queries ``cu_seqlens_q[b] : cu_seqlens_q[b + 1]`` and
     keys ``cu_seqlens_k[b] : cu_seqlens_k[b + 1]`` (int32 [B + 1]; both None: one sequence of all).  ``causal``: its queries are its last tokens,
     query i of n sees the first ``m - n + 1 + i`` of its m keys.  ``sm_scale`` must not be negative.
 
@@ -187,6 +187,8 @@ def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: 
         _need(t, n, torch.bfloat16, d)
         if t.stride(-1) != 1:
             raise ValueError(f"{n} needs unit inner stride")
+        if any(size > 1 and step == 0 for size, step in zip(t.shape, t.stride())):
+            raise ValueError(f"{n} must not be expanded")
     dev, (Tq, heads, d), Tk = q.device, q.shape, k_rope.shape[0]
     if d != 192 or heads < 1 or k_nope.shape != (Tk, heads, 128) or v.shape != (Tk, heads, 128) or k_rope.shape[1] != 64:
         raise ValueError("q must be [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64]")
