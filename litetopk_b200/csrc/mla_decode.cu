@@ -38,6 +38,7 @@ constexpr int kChunks = kD / 64;
 constexpr uint32_t kChunkBytes = kBlock * 128;              // 64 keys x 64 bf16
 constexpr uint32_t kSlotBytes = kChunks * kChunkBytes;
 constexpr int kSlots = 2;
+constexpr int kMostStartCost = 5;                           // blocks
 constexpr int kGroups = 5;                                  // a tile's chunks are loaded and given back in groups: four of 128 dims, the rope dims
 // Warps 0-7: softmax.  Who loads: one warp by TMA (bf16 rows in pages of multiples of 64), 8 by cp.async (bf16 rows in smaller pages:
 // a box is a page then, and 36 boxes a block take a warp 3400 cycles to issue), 16 through registers (packed rows).
@@ -89,7 +90,7 @@ struct Params {
   float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
   int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
   int flat_q;                     // a sequence's rows are evenly spaced: they come by TMA
-  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows;      // box_rows: of a pair's loads
+  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows, start_cost;      // box_rows: of a pair's loads
   float scale_log2;
   int epoch;
   uint32_t wait_limit;
@@ -226,13 +227,14 @@ struct Ahead {
   }
 };
 
-// Group g's share: blocks [g total / groups, (g + 1) total / groups) of all sequences' in a row.  All threads of a block.
+// Group g's share: [g total / groups, (g + 1) total / groups) of all sequences' blocks in a row, a sequence preceded by p.start_cost blocks that nobody
+// has: what its beginning, another piece for somebody, costs.  All threads of a block; ms.count is 0 before.
 template <class M>
 __device__ __forceinline__ void find_share(const Params& p, M& ms, int g, int warp, int lane) {
   const int nt = (int)blockDim.x, per = (p.B + nt - 1) / nt;
   const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += blocks_of(len_of(p, b));
+  for (int b = b0; b < b1; ++b) mine += blocks_of(len_of(p, b)) + p.start_cost;
   int incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -249,16 +251,27 @@ __device__ __forceinline__ void find_share(const Params& p, M& ms, int g, int wa
     total += ms.scan[w];
   }
   const int used = min(p.groups, total);
-  const int first = g < used ? (int)((long long)g * total / used) : total, last = g < used ? (int)((long long)(g + 1) * total / used) : total;
-  if (first >= before && first < before + mine && last > first) {
-    int at = before, b = b0;
-    for (;; ++b) {
-      const int nb = blocks_of(len_of(p, b));
-      if (first < at + nb) break;
-      at += nb;
+  if (g < used) {
+#pragma unroll
+    for (int end = 0; end < 2; ++end) {
+      const int x = (int)((long long)(g + end) * total / used);
+      if (x == total) {
+        if (threadIdx.x == 0) atomicAdd(&ms.count, total - p.B * p.start_cost);
+      } else if (x >= before && x < before + mine) {
+        int at = before, b = b0;
+        for (;; ++b) {
+          const int n = blocks_of(len_of(p, b)) + p.start_cost;
+          if (x < at + n) break;
+          at += n;
+        }
+        const int k = max(x - at - p.start_cost, 0), blocks = at - b * p.start_cost + k;      // before x
+        atomicAdd(&ms.count, end ? blocks : -blocks);
+        if (end == 0) {
+          ms.start_b = b; ms.start_k = k;
+          ms.start_pos = at; ms.total = total; ms.meta_groups = used;
+        }
+      }
     }
-    ms.start_b = b; ms.start_k = first - at; ms.count = last - first;
-    ms.start_pos = first; ms.total = total; ms.meta_groups = used;
   }
   __syncthreads();
 }
@@ -268,13 +281,10 @@ template <class M>
 __device__ __forceinline__ void write_meta(const Params& p, const M& ms, int g) {
   int4 e = make_int4(-1, 0, 0, 0);
   Walk w(ms);
-  int before = 0;
+  long long end = ms.start_pos;
   while (w.next(p)) {
-    if (w.k0 == 0 && w.k1 < w.nb) {
-      const long long end = ms.start_pos + before + w.nb;                 // behind the sequence's last block
-      e = make_int4(w.b, w.index == 0 ? 0 : 1, (int)((end * ms.meta_groups - 1) / ms.total) - g + 1, 0);
-    }
-    before += w.k1 - w.k0;
+    end += p.start_cost + w.nb;                                           // behind the sequence's last block
+    if (w.k0 == 0 && w.k1 < w.nb) e = make_int4(w.b, w.index == 0 ? 0 : 1, (int)((end * ms.meta_groups - 1) / ms.total) - g + 1, 0);
   }
   p.meta[g] = e;
 }
@@ -979,6 +989,8 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   if (B < 0 || q_len <= 0 || heads <= 0 || heads > 128 || (int64_t)q_len * heads > (1 << 20) || table_cols < 0 || n_blocks < 0 || block_size <= 0)
     return LITEDSA_ERR_SHAPE;
   if (block_size % 16 || n_blocks >= (1ll << 31) || (int64_t)table_cols * block_size >= (1ll << 31) - kBlock) return LITEDSA_ERR_UNSUPPORTED;
+  // (the blocks of all sequences are counted in 32 bits)
+  if (B * ((int64_t)table_cols * block_size / kBlock + 1 + kMostStartCost) >= (1ll << 31)) return LITEDSA_ERR_UNSUPPORTED;
   const int row = packed ? kPackedRow : 2 * kD;
   if (n_blocks > 1 && block_stride_bytes < (int64_t)block_size * row) return LITEDSA_ERR_SHAPE;
   if (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out | (uintptr_t)workspace) & 15 || block_stride_bytes % 16 ||
@@ -1003,6 +1015,9 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   }
   p.B = B; p.q_len = q_len; p.heads = heads; p.rows = q_len * heads; p.row_tiles = s.tiles; p.groups = s.groups;
   p.cols = n_blocks == 0 ? 0 : table_cols; p.block_size = block_size; p.n_blocks = (int)n_blocks;
+  // 7000 cycles at 1400 to 2600 a block of a pair, 5500 at 3000 to 3800 of a CTA (0 / 2 / 4 / 6: 256 rows, bf16 109 / 106 / 103 / 102 us; 128 rows, packed 147 /
+  // 142 / 144 / 146; 64 rows, packed 57.7 / 52.0 / 51.9 / 53.4; 16 rows, packed 44.9 / 44.4 / 46.4 / 48.9)
+  p.start_cost = s.pair && !packed ? kMostStartCost : 2;
   p.box_rows = block_size % pair::kOwnKeys == 0 ? pair::kOwnKeys : 16;
   p.scale_log2 = sm_scale * kLog2e;
   p.epoch = next_launch_epoch(); p.wait_limit = wait_limit_ticks();
