@@ -67,13 +67,17 @@ struct PairMisc {
   float top[4][64];                   // of a row's threads: maxima, sums
   float most[64];                     // what the rows' exponentials are relative to
   float corr[64], corr_peer[64];      // factors of this CTA's and of the peer's rows
-  float scale[128];                   // of the tile's rows
+  alignas(8) float scale[128];        // of the tile's rows
 };
 static_assert(sizeof(PairMisc) <= kMiscBytes, "PairMisc");
 
 // (relaxed: nothing that this thread has written is announced, and a release waited a thousand cycles for its prefetches)
 __device__ __forceinline__ void arrive_expect_cluster(uint32_t addr, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(addr), "r"(bytes) : "memory");
+}
+// a word into the peer's shared memory, counted by the barrier there: the words that a barrier has counted are there when it says so
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ uint32_t try_wait_cluster(uint64_t* bar, uint32_t parity) {
@@ -353,17 +357,19 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         if (whole) {
           const float f = sum > 0.f ? 1.f / sum : 0.f;
           ms.scale[R * cta + r] = f;
-          st_cluster_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f);
-          if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m + __log2f(sum)) * kLn2 : INFINITY;
+          st_async_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f, mapa(smem_u32(&ms.fin_full), peer));
         } else {
           p.part_ml[(long long)slot * kTile + R * cta + r] = make_float2(m, sum);
         }
       }
-      if (whole) {                                          // (both CTAs alike)
-        fence_cluster();
+      if (whole) {                                          // (both CTAs alike; the peer's factors are its own words on the barrier)
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(&ms.fin_full, 4 * R);
         softmax_sync();
-        if (threadIdx.x == 0) mbar_arrive_cluster_release(mapa(smem_u32(&ms.fin_full), peer));
         wait_cluster(&ms.fin_full, wholes++ & 1, wt, kSiteVote, kb);
+        if (h == 0 && c == 0 && row < p.rows) {
+          const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r];
+          p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m + __log2f(sum)) * kLn2 : INFINITY;
+        }
       }
       mbar_wait(&ms.slot_free[prev.slot], prev.phase, wt, kSitePv, kb);
       __syncwarp();
@@ -379,16 +385,17 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
           tmem_wait_ld();
           if (x + 16 < kTile) tmem_ld16(tmem + lane_base + kTile * c + x + 16, o[y ^ 1]);
           if (whole) {
-            // Lanes 2 i and 2 i + 1 exchange, for two dims of a row each
+            // Two rows a word, one dim; then lanes 2 i and 2 i + 1 exchange, for two dims of a row each
             const int odd = lane & 1;
+            const uint32_t order = odd ? 0x3276u : 0x5410u;
             uint32_t* dst = reinterpret_cast<uint32_t*>(p.out) + (((long long)w.b * p.rows + rt * kTile + x + odd) * kDV + (d & ~1)) / 2;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float got = __shfl_xor_sync(0xffffffffu, odd ? o[y][e] : o[y][e + 1], 1), a = odd ? got : o[y][e], b = odd ? o[y][e + 1] : got;
-              if (x + e + odd < rows) {
-                const float f = ms.scale[x + e + odd];
-                dst[e * (kDV / 2)] = f > 0.f ? bf16x2(a * f, b * f) : 0u;          // a row without keys: 0, whatever the values of others
-              }
+              const float2 f = *reinterpret_cast<const float2*>(&ms.scale[x + e]);
+              // (a row without keys: 0, whatever the values of others)
+              const uint32_t mine = bf16x2(f.x > 0.f ? o[y][e] * f.x : 0.f, f.y > 0.f ? o[y][e + 1] * f.y : 0.f);
+              const uint32_t its = __shfl_xor_sync(0xffffffffu, mine, 1);
+              if (x + e + odd < rows) dst[e * (kDV / 2)] = __byte_perm(mine, its, order);
             }
           } else {
             float* dst = p.part_o + ((long long)slot * kTile + x) * kDV + d;
