@@ -22,8 +22,8 @@
 // bf16 (exact where the scales are powers of two) and write the same tile that TMA writes for bf16 rows.
 //
 // Bound by memory up to 16 rows, by the tensor cores from 64 on.  Measured: 5 sequences of 65 to 131 thousand keys, 16 heads, bf16, 103 us = 5.5 TB/s
-// with the merge (a copy: 6.5); 32 sequences of up to 8191 packed keys, 64 heads, 57.5 us, where fifteen blocks a CTA take 3800 cycles each, the
-// latency of loads, conversion, products and softmax over two slots, and start, pieces' ends and merge 26 us.
+// with the merge (a copy: 6.5); 32 sequences of up to 8191 packed keys, 64 heads, 52 us, where fifteen blocks a CTA take 3800 cycles each, the
+// latency of loads, conversion, products and softmax over two slots, and start, pieces' ends and merge 20 us.
 //
 // A key beyond the sequence's end is in no product: its S is replaced, and its value row is zeroed before the second product, whatever its page holds.
 #include "common.cuh"
@@ -954,7 +954,7 @@ namespace lt {
 namespace decode {
 
 // Up to 64 rows a CTA has a tile, more have pairs of CTAs, 128 rows a pair.  (32 sequences of up to 8191 packed rows, 64 heads: 61 us against 67 with pairs of
-// 32 rows a CTA; 256 rows, bf16: 115 against 133 with four CTAs of 64; 128 sequences of 128 heads, packed: 160 against 215.)
+// 32 rows a CTA; 256 rows, bf16: 112 against 133 with four CTAs of 64; 128 sequences of 128 heads, packed: 160 against 215.  All with equal shares of blocks.)
 struct Shape {
   int per, tiles, groups;
   bool pair;

@@ -19,7 +19,7 @@
 // tiles first, heads one after the other so that the CTAs that run share their K and V in L2.  A call of few tiles leaves
 // most of its last wave idle: its last tiles are cut along the keys, and a second kernel merges the pieces in fp32.
 //
-// Measured: 8192 tokens x 64 heads, causal, 1047 us = 1312 TFLOP/s in a few calls, 1215 us = 1131 TFLOP/s when the power limit has brought the clock down
+// Measured: 8192 tokens x 64 heads, causal, 1047 us = 1312 TFLOP/s in a few calls, 1217 us = 1129 TFLOP/s when the power limit has brought the clock down
 // to 1.55 GHz (a library's matrix product: 1657 and 1391); 4096 tokens behind 28672, 16 heads, 957 us = 1346 TFLOP/s.  A block of a tile takes 2000
 // cycles of a CTA, of which the tensor cores compute 1300: the exponentials (128 a row and block) and the hand-overs fill the rest.
 #include "common.cuh"
