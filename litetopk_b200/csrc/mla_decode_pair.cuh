@@ -231,13 +231,11 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
       const int row = row0 + r;
       const int lim = min(w.len, w.len - p.q_len + 1 + row / p.heads), low = w.len - p.q_len + 1 + row0 / p.heads;     // low: what this CTA's first row sees
       float m = kMInit, l = 0.f;
-      auto renew = [&]() -> bool {                          // have the maxima changed?
-        if (*changes == seen) return false;
+      auto renew = [&]() {                                  // the row's maximum as the groups have settled it
         seen = *changes;
         const float now = ms.most[r];
         l *= fast_exp2(m - now);
         m = now;
-        return true;
       };
       for (int k = w.k0; k < w.k1; ++k, ++kb, prev2 = prev, prev = at, at.advance()) {
         if ((kb & 1) != c) continue;
@@ -262,7 +260,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         if (k == w.k0 + 1) {                                // (a piece's first block changes them)
           mbar_wait(&ms.decided, (kb - 1) & 1, wt, kSiteVote, kb);
           __syncwarp();
-          renew();
+          if (*changes != seen) renew();
         }
         auto must = [&]() { return first || __any_sync(0xffffffffu, mx > m + kMostOver); };
         const bool need = must();
@@ -292,16 +290,20 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         };
         // P is written as if no row needed a new maximum
         float sum = need ? 0.f : put_p();
-        bool change = group_any(c, need);
+        bool stale = false;
         if (!first) {
           mbar_wait(&ms.decided, (kb - 1) & 1, wt, kSiteVote, kb);
           __syncwarp();
-          if (renew()) {                                    // (all four warps)
-            change = group_any(c, must());
-            if (!change) {
-              sum = put_p();
-              group_any(c, false);
-            }
+          stale = *changes != seen;
+        }
+        // (what a thread finds is put to the vote before steps depend on it: where waits have given up, threads may find different things)
+        bool change = group_any(c, need || stale);
+        if (change && !first && group_any(c, stale)) {
+          renew();
+          change = group_any(c, must());
+          if (!change) {
+            sum = put_p();
+            group_any(c, false);
           }
         }
         if (change) {
@@ -346,7 +348,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         }
       }
       softmax_sync();                                       // (after the last block's change)
-      renew();
+      if (*changes != seen) renew();
       // epilogue: this CTA's dims of all of the tile's rows
       ms.top[2 * c + h][r] = l;
       const bool whole = w.whole();
