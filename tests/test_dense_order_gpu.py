@@ -33,3 +33,24 @@ def test_every_tile_is_done_once(causal, heads, lq, lk):
     a, _ = lt.mla_prefill(q[:, :1].expand(-1, heads, -1).contiguous().to(DEV), same[..., :128], rope.to(DEV), same[..., 128:], SCALE,
                           cu_seqlens_q=_cu(cu_q), cu_seqlens_k=_cu(ck), causal=causal)
     assert torch.equal(a, a[:, :1].expand(-1, heads, -1))
+
+
+@pytest.mark.parametrize("B", [33, 1000, 1100])
+@pytest.mark.parametrize("heads", [1, 3])
+def test_batches_of_many_sequences(B, heads):
+    g = _gen(B)
+    lq = torch.randint(0, 4, (B,), generator=g).tolist()
+    lq[B // 2], lq[-1] = 300, 5
+    lk = [n + int(torch.randint(0, 3, (1,), generator=g)) for n in lq]
+    q, kv, rope, cu_q, starts = _ragged(g, lq, lk, heads)
+    ck = starts + [sum(lk)]
+    kd = kv.to(DEV)
+    out, lse = lt.mla_prefill(q.to(DEV), kd[..., :128], rope.to(DEV), kd[..., 128:], SCALE, cu_seqlens_q=_cu(cu_q), cu_seqlens_k=_cu(ck))
+    pick = sorted({0, 1, 31, 32, 33 % B, B // 2, B - 2, B - 1})
+    out, lse = out.cpu(), lse.cpu()
+    for b in pick:
+        _prefill_compare(q[cu_q[b]:cu_q[b + 1]], kv, rope, [0, lq[b]], [starts[b]], [lk[b]], (out[cu_q[b]:cu_q[b + 1]], lse[cu_q[b]:cu_q[b + 1]]))
+    # every row has been written: sequences of one key hold its value
+    for b in range(B):
+        if lk[b] == 1 and lq[b] == 1:
+            assert torch.equal(out[cu_q[b]], kv[starts[b], :, 128:])
