@@ -540,9 +540,11 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
     Turn mine_to_bring{p.row_tiles, rt};
     Cursor at;
     for (int kb = 0; kb < count; ++kb, next.advance(p, lane)) {
-      if (kb >= kSlots) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&ms.slot_free[at.slot], at.phase ^ 1u, wt, kSiteFree, kb))) break;
-      }
+      // (Nothing waits for this warp, so the barrier can be two phases ahead of it and look as if it were behind; then this waits for
+      // another phase, or for the end.)
+      bool go = true;
+      while (kb >= kSlots && go && !mbar_try_wait(&ms.slot_free[at.slot], at.phase ^ 1u)) go = !wt.aborting() && *reinterpret_cast<volatile uint32_t*>(&ms.over) == 0;
+      if (!__all_sync(0xffffffffu, go)) break;
       at.advance();
       if (!mine_to_bring()) continue;
       for (int d = kb == 0 ? 0 : 2; d < 3; ++d) {

@@ -115,3 +115,18 @@ def test_queries_with_strides_and_rows_left_alone():
     keep = [0, 63, 64, 69]
     _compare(q[:, :, keep], lens, 32, table, rows, (got[0][:, :, keep].contiguous(), got[1][:, :, keep].contiguous()))
     assert bool((out[::3] == 5).all()) and bool((lse[::3] == 5).all())
+
+
+def test_many_short_sequences_of_packed_rows():
+    # pieces of a block or two: whoever looks ahead reads a length for each, while the others are done with several
+    g = _gen(51)
+    B, heads, longest = 3000, 128, 129
+    cache, table, rows = _cache(g, [longest] * 8, 16, True, poison=False)
+    table = table.repeat(B // 8, 1)
+    lens = torch.where(torch.arange(B) % 50 == 0, longest, torch.randint(0, 3, (B,), generator=g))
+    q = _bf16(g, B, 1, heads, 576)
+    for _ in range(3):
+        out, lse = lt.mla_decode(q.to(DEV), cache.to(DEV), table.to(DEV), _lens(lens.tolist()), SCALE)
+        assert lt.mla_decode_status(reset=True)[0] == 0
+    keep, picks = [0, 64, 127], [0, 1, 2, 49, 50, 1500, 2998, 2999]
+    _compare(q[:, :, keep], lens.tolist(), 16, table, rows, (out[:, :, keep].contiguous(), lse[:, :, keep].contiguous()), picks)
