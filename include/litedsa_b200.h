@@ -485,8 +485,9 @@ int litedsa_append_kv(const void* kv_c, int64_t kv_c_stride, const void* k_rope,
  *               Lengths are clamped to [0, table_cols * block_size]; blocks outside the cache read as zeros
  *   out         [B, q_len, heads, 512] bf16, lse [B, q_len, heads] fp32, dense
  *   workspace   litedsa_mla_decode_workspace(q_len, heads) bytes on the current device, 16-byte aligned; it holds nothing between calls
- * A row that sees no key gets out = 0, lse = +inf.  Keys behind a sequence's end are in no result, whatever their rows hold; a
- * value that is infinite or NaN can reach the earlier of the sequence's new tokens, although they may not see it.
+ * A row that sees no key, or whose scores are all -inf, gets out = 0, lse = +inf; one with a score that is NaN or +inf gets NaN in both.  Keys
+ * behind a sequence's end are in no result, whatever their rows hold; a value that is infinite or NaN can reach the earlier of the sequence's new
+ * tokens, although they may not see it.
  */
 int64_t litedsa_mla_decode_workspace(int q_len, int heads);
 int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -508,7 +509,8 @@ int litedsa_mla_decode_status(int* out4_host, int reset);
  *   out     [Tq, heads, 128] bf16, lse [Tq, heads] fp32, dense
  *   workspace   litedsa_mla_prefill_workspace(Tq, Tk, heads) bytes (0 for most sizes) on the current device, 16-byte
  *           aligned; it holds nothing between calls
- * sm_scale is not negative.  A row that sees no key gets out = 0, lse = +inf.  Keys of other sequences and behind the last one are in no result,
+ * sm_scale is not negative.  A row that sees no key, or whose scores are all -inf, gets out = 0, lse = +inf; one with a score that is NaN or +inf
+ * gets NaN in both.  Keys of other sequences and behind the last one are in no result,
  * whatever they hold; a value that is infinite or NaN can reach the rows of its sequence that share a block of 128 keys
  * with it, although they may not see it.
  */

@@ -26,6 +26,8 @@
 // latency of loads, conversion, products and softmax over two slots, and start, pieces' ends and merge 20 us.
 //
 // A key beyond the sequence's end is in no product: its S is replaced, and its value row is zeroed before the second product, whatever its page holds.
+// A row's sum of exponentials is 0 where it sees no key, and NaN where a score is NaN or +infinity: maxima pass NaN over, sums and products keep it, and the
+// ends and the merge ask for a sum of 0, not for a positive one.
 #include "common.cuh"
 #include "tensor_map.cuh"
 
@@ -462,9 +464,9 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         for (int i = 0; i < 2; ++i) {
           const int r = r0 + 8 * i, row = rt * kRows + r;
           const float sum = ms.sum[0][r] + ms.sum[1][r];
-          ms.corr[r] = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
+          ms.corr[r] = whole ? (sum != 0.f ? 1.f / sum : 0.f) : 1.f;
           if (whole) {
-            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m[i] + __log2f(sum)) * kLn2 : INFINITY;
+            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum != 0.f ? (m[i] + __log2f(sum)) * kLn2 : INFINITY;
           } else {
             p.part_ml[(long long)slot * kRows + r] = make_float2(m[i], sum);
           }
@@ -488,7 +490,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
             for (int e = 0; e < 16; ++e)
               if (r + e < rows) {
                 const float f = ms.corr[r + e];
-                dst[e * kDV] = __float2bfloat16(f > 0.f ? o[u][e] * f : 0.f);      // a row without keys: 0, whatever the values of others
+                dst[e * kDV] = __float2bfloat16(f != 0.f ? o[u][e] * f : 0.f);     // a row without keys: 0, whatever the values of others
               }
           } else {
             float* dst = p.part_o + ((long long)slot * kRows + r) * kDV + d;
@@ -792,7 +794,7 @@ __device__ __forceinline__ void add_parts(const Params& p, int kRows, int g, con
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (!(ml[u].y > 0.f)) continue;                  // beyond the list, or a part without keys
+      if (ml[u].y == 0.f) continue;                    // beyond the list, or a part without keys
       const float f = fast_exp2(ml[u].x - m);
       l += f * ml[u].y;
 #pragma unroll
@@ -832,7 +834,7 @@ __device__ __forceinline__ void add_few(const Params& p, int kRows, int g, const
 #pragma unroll
     for (int u = 0; u < 3; ++u) {
       const float f = __shfl_sync(0xffffffffu, w, i0 + u), y = __shfl_sync(0xffffffffu, ml.y, i0 + u);
-      if (!(y > 0.f)) continue;                        // beyond the list, or a part without keys
+      if (y == 0.f) continue;                          // beyond the list, or a part without keys
       l += f * y;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -905,11 +907,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps, 2) mla_decode_merge_kernel(c
       }
       const long long to = (long long)e.x * p.rows + row;
       if (alone) {
-        const float f = l > 0.f ? 1.f / l : 0.f;
+        const float f = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           reinterpret_cast<uint2*>(p.out)[to * (kDV / 4) + 32 * c + lane] = make_uint2(bf16x2(a[c].x * f, a[c].y * f), bf16x2(a[c].z * f, a[c].w * f));
-        if (lane == 0) p.lse[to] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+        if (lane == 0) p.lse[to] = l != 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
       } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[warp][32 * c + lane] = a[c];
@@ -924,9 +926,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps, 2) mla_decode_merge_kernel(c
             o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
             l += sum_l[w];
           }
-          const float f = l > 0.f ? 1.f / l : 0.f;
+          const float f = l != 0.f ? 1.f / l : 0.f;
           reinterpret_cast<uint2*>(p.out)[to * (kDV / 4) + threadIdx.x] = make_uint2(bf16x2(o.x * f, o.y * f), bf16x2(o.z * f, o.w * f));
-          if (threadIdx.x == 0) p.lse[to] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+          if (threadIdx.x == 0) p.lse[to] = l != 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
         }
         __syncthreads();
       }

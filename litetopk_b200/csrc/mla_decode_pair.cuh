@@ -357,7 +357,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
       if (h == 0 && c == 0) {
         const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r];
         if (whole) {
-          const float f = sum > 0.f ? 1.f / sum : 0.f;
+          const float f = sum != 0.f ? 1.f / sum : 0.f;
           ms.scale[R * cta + r] = f;
           st_async_f32(mapa(smem_u32(&ms.scale[R * cta + r]), peer), f, mapa(smem_u32(&ms.fin_full), peer));
         } else {
@@ -370,7 +370,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         wait_cluster(&ms.fin_full, wholes++ & 1, wt, kSiteVote, kb);
         if (h == 0 && c == 0 && row < p.rows) {
           const float sum = ms.top[0][r] + ms.top[1][r] + ms.top[2][r] + ms.top[3][r];
-          p.lse[(long long)w.b * p.rows + row] = sum > 0.f ? (m + __log2f(sum)) * kLn2 : INFINITY;
+          p.lse[(long long)w.b * p.rows + row] = sum != 0.f ? (m + __log2f(sum)) * kLn2 : INFINITY;
         }
       }
       mbar_wait(&ms.slot_free[prev.slot], prev.phase, wt, kSitePv, kb);
@@ -395,7 +395,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
             for (int e = 0; e < 16; e += 2) {
               const float2 f = *reinterpret_cast<const float2*>(&ms.scale[x + e]);
               // (a row without keys: 0, whatever the values of others)
-              const uint32_t mine = bf16x2(f.x > 0.f ? o[y][e] * f.x : 0.f, f.y > 0.f ? o[y][e + 1] * f.y : 0.f);
+              const uint32_t mine = bf16x2(f.x != 0.f ? o[y][e] * f.x : 0.f, f.y != 0.f ? o[y][e + 1] * f.y : 0.f);
               const uint32_t its = __shfl_xor_sync(0xffffffffu, mine, 1);
               if (x + e + odd < rows) dst[e * (kDV / 2)] = __byte_perm(mine, its, order);
             }

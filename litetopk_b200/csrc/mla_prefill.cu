@@ -421,9 +421,9 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         ++no;
         tc_fence_after();
       }
-      const float f = l > 0.f ? 1.f / l : 0.f;
+      const float f = l != 0.f ? 1.f / l : 0.f;
       if (mine) {
-        if (k.part < 0) p.lse[row] = l > 0.f ? (m * c + __log2f(l)) * kLn2 : INFINITY;
+        if (k.part < 0) p.lse[row] = l != 0.f ? (m * c + __log2f(l)) * kLn2 : INFINITY;     // (NaN: a score was none)
         else p.part_ml[prow] = make_float2(m * c, l);
       }
       if (k.part < 0) {
@@ -440,7 +440,7 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             for (int y = 0; y < 4; ++y) {
               uint32_t w[4];
 #pragma unroll
-              for (int z = 0; z < 4; ++z) w[z] = l > 0.f ? bf16x2(o[8 * y + 2 * z] * f, o[8 * y + 2 * z + 1] * f) : 0u;   // without keys: 0
+              for (int z = 0; z < 4; ++z) w[z] = l != 0.f ? bf16x2(o[8 * y + 2 * z] * f, o[8 * y + 2 * z + 1] * f) : 0u;   // without keys: 0
               dst[4 * x + y] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_prefill_merge_kernel(con
   float m = kMInit;
   for (int i = lane; i < cut.pieces; i += 32) {
     const float2 ml = __ldcg(p.part_ml + base + (long long)i * kPair);
-    if (ml.y > 0.f) m = fmaxf(m, ml.x);
+    if (ml.y != 0.f) m = fmaxf(m, ml.x);
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
@@ -686,16 +686,16 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_prefill_merge_kernel(con
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      if (!(ml[u].y > 0.f)) continue;                         // beyond the list, or a piece without keys for this row
+      if (ml[u].y == 0.f) continue;                           // beyond the list, or a piece without keys for this row
       const float f = fast_exp2(ml[u].x - m);
       l += f * ml[u].y;
       a.x += f * v[u].x; a.y += f * v[u].y; a.z += f * v[u].z; a.w += f * v[u].w;
     }
   }
-  const float f = l > 0.f ? 1.f / l : 0.f;
+  const float f = l != 0.f ? 1.f / l : 0.f;
   const long long row = (long long)(k.q0 + rr) * p.heads + k.head;
   reinterpret_cast<uint2*>(p.out + row * (2 * kDV))[lane] = make_uint2(bf16x2(a.x * f, a.y * f), bf16x2(a.z * f, a.w * f));
-  if (lane == 0) p.lse[row] = l > 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
+  if (lane == 0) p.lse[row] = l != 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
 }
 
 // Pieces that a call's workspace holds: none where its tiles are known to be many, or its sequences too short to be cut.

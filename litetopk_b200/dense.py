@@ -113,7 +113,8 @@ def mla_decode(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tenso
     ``seq_lens - q_len + 1 + j``.  Keys are the 576 dims of a row, values its first 512.
 
     Returns ``(out [B, (q_len,) heads, 512] bf16, lse [B, (q_len,) heads] f32)``, written into ``out`` / ``lse`` when given
-    (contiguous).  A row that sees no key: out = 0, lse = +inf.  Lengths are clamped to what a row of the table can hold.
+    (contiguous).  A row that sees no key: out = 0, lse = +inf; one with a score that is NaN or +inf: NaN in both.  Lengths are clamped to what a
+    row of the table can hold.  A cached value that is infinite or NaN can reach the earlier of its sequence's new tokens, although they may not see it.
     """
     if out is None and lse is None and (host := _lib.host()) is not None:
         r = host.mla_decode(q, kv_cache, block_table, seq_lens, sm_scale)
@@ -175,7 +176,8 @@ def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: 
     query i of n sees the first ``m - n + 1 + i`` of its m keys.  ``sm_scale`` must not be negative.
 
     Returns ``(out [Tq, heads, 128] bf16, lse [Tq, heads] f32)``, written into ``out`` / ``lse`` when given (contiguous).  A row that sees
-    no key: out = 0, lse = +inf.  Rows that are no sequence's (behind ``cu_seqlens_q[-1]``) are not written.
+    no key: out = 0, lse = +inf; one with a score that is NaN or +inf: NaN in both.  A value that is infinite or NaN can reach rows of its sequence
+    that share a block of 128 keys with it, although they may not see it.  Rows that are no sequence's (behind ``cu_seqlens_q[-1]``) are not written.
     """
     if out is None and lse is None and (host := _lib.host()) is not None:
         r = host.mla_prefill(q, k_nope, k_rope, v, sm_scale, cu_seqlens_q, cu_seqlens_k, causal)
