@@ -23,6 +23,8 @@ LIB = OUT_DIR / "liblitedsa_b200.so"
 HOST_SRC = CSRC / "host_binding.cpp"
 SOURCES = ["abi.cu", "union_qm.cu", "attn_fp8.cu", "prep.cu", "noalloc.cu", "attn_dsv4.cu", "attn_bf16.cu", "peak_probe.cu", "index_topk.cu",
            "prefill.cu", "append_kv.cu", "mla_decode.cu", "mla_prefill.cu"]
+# Rotation and quantisation of what a cache holds keep numbers below 2^-126, which fast-math takes for 0
+FLAGS = {"append_kv.cu": ["-ftz=false"]}
 
 
 def _nvcc() -> str:
@@ -84,7 +86,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     for src in sources():
         obj = OUT_DIR / (src.stem + ".o")
         cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
-               "-std=c++17", "-use_fast_math", "--compiler-options=-fPIC", "-c", str(src),
+               "-std=c++17", "-use_fast_math", *FLAGS.get(src.name, []), "--compiler-options=-fPIC", "-c", str(src),
                "-o", str(obj)]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")

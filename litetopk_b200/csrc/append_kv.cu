@@ -6,6 +6,8 @@
 //   packed    512 e4m3 codes | 4 fp32 scales | 64 bf16: scale = the smallest power of two that brings a group's 128 dims into
 //             +-448, so that code x scale is exact in bf16 and attention over the row rounds nothing again
 //
+// Compiled without flushing to zero: numbers below 2^-126 are turned and packed like any others.
+//
 // Element-wise and bound by memory; a few tokens by latency, so a token is a block of its own: up to eight warps of it rotate heads
 // (eight lanes a head, eight heads a warp), the last one has the cache row, sixteen latent dims a lane, so that a group's
 // maximum is three shuffles.  Everything is read and written once, 16 bytes an access, neighbouring lanes neighbouring bytes.
