@@ -698,11 +698,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_prefill_merge_kernel(con
   if (lane == 0) p.lse[row] = l != 0.f ? (m + __log2f(l)) * kLn2 : INFINITY;
 }
 
-// Pieces that a call's workspace holds: none where its tiles are known to be many, or its sequences too short to be cut.
+// Pieces that a call's workspace holds: none where its tiles are known to be many, or its sequences too short to be cut; else what cut_of can
+// come to: pieces of two blocks, of at most a tile a query and head and of fewer tiles than CTAs.
 static int pieces_of(int Tq, int Tk, int heads) {
-  const int ctas = sm_count();
+  const int ctas = sm_count(), blocks = blocks_seen(Tk);
   const int64_t tiles = (int64_t)((Tq + kPair - 1) / kPair) * heads;
-  return tiles > 4 * ctas || blocks_seen(Tk) < 4 ? 0 : 4 * ctas;
+  if (tiles > 4 * ctas || blocks < 4) return 0;
+  return (int)min((int64_t)4 * ctas, min((int64_t)Tq * heads, (int64_t)max(ctas - 1, 1)) * (blocks / 2));
 }
 
 }  // namespace prefill
