@@ -328,6 +328,11 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
   const unsigned long long t0 = globaltimer_ns();
   while (!mbar_test(bar, parity) && globaltimer_ns() - t0 < kDrainLimitNs) {}
 }
+// The same where what is in flight is counted by another block's barriers: that limit as a time
+__device__ __forceinline__ void drain_uncounted() {
+  const unsigned long long t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < kDrainLimitNs) {}
+}
 
 // release at cluster scope: orders this thread's earlier (distributed) shared-memory stores
 __device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_addr) {

@@ -508,10 +508,8 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
     const uint32_t a_ready = mapa(smem_u32(&ms.q_ready), 0);
     Walk w(ms);
     const uint64_t pol = l2_policy_evict_first();
-    bool ok = true;
-    int asked = 0;
     while (w.next(p)) {
-      if (w.index > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.q_free, (w.index - 1) & 1, wt, kSiteQ, w.index)))) break;
+      if (w.index > 0 && !__all_sync(0xffffffffu, mbar_wait(&ms.q_free, (w.index - 1) & 1, wt, kSiteQ, w.index))) break;
       if (p.flat_q) {
         if (lane == 0) arrive_expect_cluster(a_ready, kChunks * PL::kQChunk);
         __syncwarp();
@@ -529,10 +527,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(a_ready);
       }
-      ++asked;
     }
-    if (!ok && asked > 0 && lane == 0 && cta == 0) mbar_drain(&ms.q_ready, (asked - 1) & 1);        // given up: what is in flight lands first
-    __syncwarp();
   } else if (kLoad == kPacked && warp == kWarpBring) {
     // ------------------------------------------------------------ this CTA's keys into L2, two blocks ahead of the converting warps
     const int count = ms.count;
@@ -615,7 +610,6 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         if (!is_v && src != nullptr && lane == 0 && (rows_own < kOwnKeys || second == 0)) l2_prefetch_1d(src, (uint32_t)(n * kRowBytes));
       };
       const uint64_t pol = l2_policy_evict_first();
-      int asked = 0;
       // what the lane requests of a block
       const int chunk = is_v ? lane & 3 : boxes == 1 ? lane + 5 * second : lane;
       const bool mine = is_v ? lane < 4 * boxes : boxes == 1 ? (second ? lane < 4 : lane < 5) : lane < kChunks;
@@ -632,7 +626,6 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
           if (mine)
             tma_load_3d_pair_hint(slot + (chunk0 + chunk) * kChunk + (first_row + 16 * box) * 128, &map_kv, dim0 + 64 * chunk, box ? row2 : row1,
                                   box ? page2 : page1, a_full + 8u * at.slot, pol);
-          asked = kb + 1;
         } else {
           // zeros behind a sequence's end: 0 x NaN is NaN
           for (int x = second == 0 || boxes > 1 ? 0 : rows_own; x < rows_own; x += 16) {
@@ -652,7 +645,6 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
         }
         at.advance();
       }
-      if (!ok && asked > 0) __nanosleep(100000);            // given up: what is in flight lands first (some microseconds; its barrier is the leader's)
     } else if (!is_v) {
       // Of each 128 dims eight lanes have 16 codes of a row each, four rows at a time.  A group's registers are loaded for the next
       // block as soon as they are converted for this one, from L2, where the rows were brought a block before.
@@ -734,6 +726,9 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
   if (warp == kWarpQk && rt == 0 && cta == 0 && lane == 0 && p.meta) write_meta(p, ms, g);
   tc_fence_before();
   __syncthreads();
+  // Given up: what is in flight lands before either CTA's memory goes.  (Loads, factors and commits are counted by barriers of which some are the other
+  // CTA's and may never complete.  A CTA that has not given up has nothing in flight: its last block's second product is complete.)
+  if (threadIdx.x == 0 && wt.aborting()) drain_uncounted();
   cluster_sync_all();                                       // nothing of this CTA is in use by the other
   tc_fence_after();
   if (warp == kWarpQk) tmem_dealloc_pair(tmem, PL::kTmemCols);

@@ -1,0 +1,61 @@
+"""Waits that run out in the dense attention kernels: a call returns and says so in its status, and the next call is as right as any.
+
+With the shortest limit a wait gives up that takes longer than some milliseconds.  Some legitimately do where a sequence is long enough:
+whoever brings the next piece's queries waits for as long as the present piece takes.  Its keys are a few pages, over and over.
+"""
+import pytest
+import torch
+
+import litetopk_b200 as lt
+from litetopk_b200 import api
+from test_dense_gpu import DEV, SCALE
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def limit():
+    yield api.set_wait_limit_ns
+    api.set_wait_limit_ns(0)
+
+
+def _gives_up_and_recovers(limit, call, status, sites):
+    right = call()
+    assert status(reset=True)[0] == 0
+    limit(1)
+    call()
+    assert status(reset=True)[0] in sites
+    limit(0)
+    again = call()
+    assert status(reset=True)[0] == 0
+    assert all(torch.equal(a, b) for a, b in zip(right, again))
+
+
+def _decode(heads, block, packed, sequences, blocks, rising=False):
+    g = torch.Generator(device=DEV).manual_seed(heads)
+    pages, cols = 2048 // block, 64 * blocks // block
+    if packed:
+        cache = torch.randint(0, 126, (pages, block, 656), generator=g, device=DEV).to(torch.uint8)
+        cache[..., 512:528] = torch.ones(4, device=DEV).view(torch.uint8)
+        cache[..., 528:] = torch.randn((pages, block, 64), generator=g, device=DEV).bfloat16().view(torch.uint8)
+    else:
+        cache = torch.randn((pages, block, 576), generator=g, device=DEV).bfloat16()
+    table = torch.randint(0, pages, (sequences, cols), generator=g, device=DEV).int()
+    lens = torch.full((sequences,), 64 * blocks, dtype=torch.int32, device=DEV)
+    q = torch.randn((sequences, heads, 576), generator=g, device=DEV).bfloat16()
+    if rising:                                         # page after page, each with scores far above the one before: maxima move all the time
+        table = (torch.arange(cols, device=DEV) * pages // cols).int().repeat(sequences, 1)
+        ramp = (torch.arange(pages, device=DEV) * (60 * block / 64)).bfloat16()[:, None]
+        if packed:
+            cache[..., 528:530] = ramp.view(torch.uint8).view(pages, 1, 2)
+        else:
+            cache[..., 512] = ramp
+        q[..., 512] = 8
+    return lambda: lt.mla_decode(q, cache, table, lens, SCALE)
+
+
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("packed,block", [(False, 64), (False, 16), (True, 64)])
+def test_decode_of_many_rows(limit, packed, block, rising):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    _gives_up_and_recovers(limit, _decode(128, block, packed, sms, 6000, rising), lt.mla_decode_status, range(1, 10))
