@@ -355,7 +355,8 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
     Walk w(ms);
     int kb = 0;
-    // A wait here that gives up is passed like any other: the warps meet at named barriers, so they take the same steps.
+    // A wait here that gives up is passed like any other: the warps meet at named barriers, so they take the same steps.  (A warp's lanes may give up at
+    // different times: they meet again before the warp reads tensor memory.)
     bool more = w.next(p);
     while (more) {
       // rows' limits
@@ -369,6 +370,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       float m[2] = {kMInit, kMInit}, l[2] = {0.f, 0.f};
       for (int k = w.k0; k < w.k1; ++k, ++kb) {
         mbar_wait(&ms.s_ready[kb & 1], (kb >> 1) & 1, wt, kSiteS, kb);
+        __syncwarp();
         tc_fence_after();
         float v[16];
         float mx[2] = {-INFINITY, -INFINITY};
@@ -408,6 +410,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
           if (!first) {
             softmax_sync();
             mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+            __syncwarp();
             tc_fence_after();
 #pragma unroll 1
             for (int c = 2 * kRows * half; c < 2 * kRows * (half + 1); c += 16) {
@@ -473,6 +476,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         }
       softmax_sync();
       mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
+      __syncwarp();
       tc_fence_after();
       const int rows = min(kRows, p.rows - rt * kRows);
       float o[2][16];

@@ -59,3 +59,17 @@ def _decode(heads, block, packed, sequences, blocks, rising=False):
 def test_decode_of_many_rows(limit, packed, block, rising):
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     _gives_up_and_recovers(limit, _decode(128, block, packed, sms, 6000, rising), lt.mla_decode_status, range(1, 10))
+
+
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("heads", [16, 64])
+@pytest.mark.parametrize("packed,block", [(False, 64), (False, 16), (True, 64)])
+def test_decode_of_few_rows(limit, packed, block, heads, rising):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    _gives_up_and_recovers(limit, _decode(heads, block, packed, 2 * sms, 8000, rising), lt.mla_decode_status, range(1, 10))
+
+
+def test_decode_with_a_cut_sequence(limit):
+    # parts of a launch that gave up are merged like any others; nothing of them is left afterwards
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    _gives_up_and_recovers(limit, _decode(32, 64, False, 2 * sms + 5, 8000), lt.mla_decode_status, range(1, 10))
