@@ -68,7 +68,7 @@ struct Params {
   float* lse;                  // [Tq, heads]
   float* part_o;               // [piece][256][128]
   float2* part_ml;             // [piece][256]: (maximum, sum)
-  int4* plan;                  // (tiles, first tile that is cut, pieces a tile, 0) for the merge
+  int4* plan;                  // (tiles, first tile that is cut, pieces a tile, this launch) for the merge
   int B, Tq, Tk, heads, ctas, causal, max_pieces;
   float scale_log2;
   int epoch;
@@ -561,7 +561,7 @@ mla_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     int w = (int)blockIdx.x, block0 = 0, asked[2] = {0, 0}, nq[2] = {0, 0}, clc_asked = 0, clc_got = 0;
     bool ok = true;
     for (int it = 0; ok;) {
-      if (w == 0 && lane == 0 && p.plan) *p.plan = make_int4(tiles, cut.whole, cut.pieces, 0);
+      if (w == 0 && lane == 0 && p.plan) *p.plan = make_int4(tiles, cut.whole, cut.pieces, p.epoch);
       Work k;
       k.live = 0;
       if (w >= 0) k = work_of(w, order, cut, p, lane);
@@ -659,6 +659,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) mla_prefill_merge_kernel(con
   const int4 plan = __ldcg(p.plan);
   const Cut cut{plan.y, plan.z};
   const int w0 = cut.whole + (int)blockIdx.y * cut.pieces, rr = (int)blockIdx.x * kMergeWarps + warp;
+  if (plan.w != p.epoch) return;                              // a launch that gave up before it had a plan: whatever lies there is none
   if (cut.pieces < 2 || cut.whole + (int)blockIdx.y >= plan.x * p.heads) return;
   const Work k = work_of(w0, order_of(plan.x, 0, p, lane), cut, p, lane);
   if (!k.live || rr >= k.rows) return;

@@ -73,3 +73,24 @@ def test_decode_with_a_cut_sequence(limit):
     # parts of a launch that gave up are merged like any others; nothing of them is left afterwards
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     _gives_up_and_recovers(limit, _decode(32, 64, False, 2 * sms + 5, 8000), lt.mla_decode_status, range(1, 10))
+
+
+def _prefill(heads, Tk):
+    # (a key's heads begin a row apart in one and the same memory)
+    g = torch.Generator(device=DEV).manual_seed(heads)
+    rows = [torch.randn((Tk + heads, 128), generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+    k, v = (x.as_strided((Tk, heads, 128), (128, 128, 1)) for x in rows)
+    q = torch.randn((1, heads, 192), generator=g, device=DEV).bfloat16()
+    rope = torch.randn((Tk, 64), generator=g, device=DEV, dtype=torch.bfloat16)
+    return lambda: lt.mla_prefill(q, k, rope, v, SCALE)
+
+
+def test_prefill(limit):
+    # as many tiles as multiprocessors: whole.  The second tile has no query, so its warps wait for the next work as long as this one takes
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    _gives_up_and_recovers(limit, _prefill(sms, 128 * 6000), lt.mla_prefill_status, range(1, 11))
+
+
+def test_prefill_of_tiles_that_are_cut(limit):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    _gives_up_and_recovers(limit, _prefill(sms * 2 // 3, 128 * 24000), lt.mla_prefill_status, range(1, 11))
