@@ -157,6 +157,15 @@ struct Ring {
   }
 };
 
+// A launch that cannot be: NaN in all results, and no parts for the merge
+__device__ __forceinline__ void refuse(const Params& p) {
+  const long long i0 = (long long)blockIdx.x * blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x, rows = (long long)p.B * p.rows;
+  for (long long i = i0; i < rows * (kDV / 2); i += step) reinterpret_cast<uint32_t*>(p.out)[i] = 0x7fff7fffu;
+  for (long long i = i0; i < rows; i += step) p.lse[i] = __uint_as_float(0x7fffffffu);
+  if (p.meta)
+    for (long long i = i0; i < p.groups; i += step) p.meta[i] = make_int4(-1, 0, 0, 0);
+}
+
 template <Load kLoad>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads<kLoad>, 1)
 mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_constant__ CUtensorMap map_q, const Params p) {
@@ -167,6 +176,7 @@ mla_decode_pair_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_
   // Swizzled tiles.  There is no room for rounding; the driver has put the base on such a boundary so far, in both CTAs alike.
   if ((sbase & 1023u) != 0) {
     pdl_wait();
+    refuse(p);
     if (threadIdx.x == 0) Waiter{g_status, p.epoch, 0}.fail(kSiteAlign, (int)(sbase & 1023u));
     return;
   }
