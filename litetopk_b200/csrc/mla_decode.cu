@@ -13,9 +13,9 @@
 // room for S, but R columns for each of four times 128 lanes of dims; and because its cost then follows the rows that exist.  The row
 // statistics stay per thread (S has rows on lanes), and only the rare rescaling of O wants them by column, from shared memory.
 //
-// Work is cut along the keys: the blocks of all sequences in a row are dealt to groups of CTAs in equal shares (a group: one
-// CTA per 64 rows of a sequence, which read the same keys at the same time, once from memory and again from L2).  A share's pieces
-// of sequences that other groups have parts of go to a workspace in fp32 and are merged by a second kernel.  Every size but those of the
+// Work is cut along the keys: the blocks of all sequences in a row are dealt to groups in equal shares (a group: a CTA; of more than 64 rows
+// as many pairs of CTAs as a sequence has tiles of 128, which read the same keys at about the same time, once from memory and again from L2).  A share's
+// pieces of sequences that other groups have parts of go to a workspace in fp32 and are merged by a second kernel.  Every size but those of the
 // tensors is read on the device, so captured calls follow new lengths.
 //
 // Packed rows (512 e4m3 codes, four fp32 scales, 64 bf16) pass through registers: sixteen warps load a block ahead, convert it to
@@ -88,11 +88,11 @@ struct Params {
   const int32_t* lens;
   uint8_t* out;                   // [B, rows, 512] bf16
   float* lse;                     // [B, rows]
-  float* part_o;                  // [CTA][2][kRows][512]
-  float2* part_ml;                // [CTA][2][kRows]: (maximum, sum)
+  float* part_o;                  // [CTA or pair][2][rows of its tile][512]
+  float2* part_ml;                // [CTA or pair][2][rows of its tile]: (maximum, sum)
   int4* meta;                     // [groups]: (sequence, slot, parts, 0) of a sequence that begins here and ends in another group, or (-1, ..)
   int flat_q;                     // a sequence's rows are evenly spaced: they come by TMA
-  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows, start_cost;      // box_rows: of a pair's loads
+  int B, q_len, heads, rows, row_tiles, groups, cols, block_size, n_blocks, box_rows, start_cost;      // row_tiles: pairs to a group; box_rows: of a pair's loads
   float scale_log2;
   int epoch;
   uint32_t wait_limit;
@@ -122,15 +122,6 @@ struct PageAt {
     page += add_page;
     row += add_row;
     if (row >= size) { row -= size; ++page; }
-  }
-};
-// true once in `every` calls, the first time after `from` of them
-struct Turn {
-  int every, left;
-  __device__ __forceinline__ bool operator()() {
-    if (left-- > 0) return false;
-    left = every - 1;
-    return true;
   }
 };
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -324,7 +315,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
   Misc& ms = *reinterpret_cast<Misc*>(sm + PL::kOffMisc);
   const BlockWaiter wt{&ms.left, p.wait_limit};
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int g = (int)blockIdx.x / p.row_tiles, rt = (int)blockIdx.x - g * p.row_tiles;
+  const int g = (int)blockIdx.x;
   pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i)
@@ -363,10 +354,9 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       int lim[2], low;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = rt * kRows + r0 + 8 * i;
-        lim[i] = min(w.len, w.len - p.q_len + 1 + row / p.heads);
+        lim[i] = min(w.len, w.len - p.q_len + 1 + (r0 + 8 * i) / p.heads);
       }
-      low = w.len - p.q_len + 1 + rt * kRows / p.heads;                   // what the tile's first row sees
+      low = w.len - p.q_len + 1;                                          // what the first row sees
       float m[2] = {kMInit, kMInit}, l[2] = {0.f, 0.f};
       for (int k = w.k0; k < w.k1; ++k, ++kb) {
         mbar_wait(&ms.s_ready[kb & 1], (kb >> 1) & 1, wt, kSiteS, kb);
@@ -460,16 +450,16 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         if (live && qd == 0) ms.sum[half][r0 + 8 * i] = l[i];
       }
       const bool whole = w.whole();
-      const int slot = (int)blockIdx.x * 2 + (w.index == 0 ? 0 : 1);
+      const int slot = g * 2 + (w.index == 0 ? 0 : 1);
       softmax_sync();
       if (live && half == 0 && qd == 0)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int r = r0 + 8 * i, row = rt * kRows + r;
+          const int r = r0 + 8 * i;
           const float sum = ms.sum[0][r] + ms.sum[1][r];
           ms.corr[r] = whole ? (sum != 0.f ? 1.f / sum : 0.f) : 1.f;
           if (whole) {
-            if (row < p.rows) p.lse[(long long)w.b * p.rows + row] = sum != 0.f ? (m[i] + __log2f(sum)) * kLn2 : INFINITY;
+            if (r < p.rows) p.lse[(long long)w.b * p.rows + r] = sum != 0.f ? (m[i] + __log2f(sum)) * kLn2 : INFINITY;
           } else {
             p.part_ml[(long long)slot * kRows + r] = make_float2(m[i], sum);
           }
@@ -478,7 +468,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       mbar_wait(&ms.kv_free[(kb - 1) & 1][kGroups - 1], ((kb - 1) >> 1) & 1, wt, kSitePv, kb);
       __syncwarp();
       tc_fence_after();
-      const int rows = min(kRows, p.rows - rt * kRows);
       float o[2][16];
       tmem_ld16(tmem + lane_base + 2 * kRows * half, o[0]);
 #pragma unroll 1
@@ -489,10 +478,10 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
           tmem_wait_ld();
           if (c + 16 < 2 * kRows * (half + 1)) tmem_ld16(tmem + lane_base + c + 16, o[u ^ 1]);
           if (whole) {
-            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + rt * kRows + r) * kDV + d;
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((long long)w.b * p.rows + r) * kDV + d;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (r + e < rows) {
+              if (r + e < p.rows) {
                 const float f = ms.corr[r + e];
                 dst[e * kDV] = __float2bfloat16(f != 0.f ? o[u][e] * f : 0.f);     // a row without keys: 0, whatever the values of others
               }
@@ -500,7 +489,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
             float* dst = p.part_o + ((long long)slot * kRows + r) * kDV + d;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (r + e < rows) dst[e * kDV] = o[u][e];
+              if (r + e < p.rows) dst[e * kDV] = o[u][e];
           }
         }
       }
@@ -584,11 +573,11 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       if (p.flat_q) {
         if (lane == 0) mbar_arrive_expect_tx(&ms.q_ready, kChunks * PL::kQChunk);
         __syncwarp();
-        if (lane < kChunks) tma_load_3d_hint(sbase + PL::kOffQ + lane * PL::kQChunk, &map_q, 64 * lane, rt * kRows, w.b, &ms.q_ready, pol);
+        if (lane < kChunks) tma_load_3d_hint(sbase + PL::kOffQ + lane * PL::kQChunk, &map_q, 64 * lane, 0, w.b, &ms.q_ready, pol);
       } else {
         for (int r = 0; r < kRows; ++r) {
-          const int row = rt * kRows + r, j = row / p.heads, h = row - j * p.heads;
-          const bool in = row < p.rows;
+          const int j = r / p.heads, h = r - j * p.heads;
+          const bool in = r < p.rows;
           const uint8_t* src = p.q + (in ? w.b * p.q_b + j * p.q_j + h * p.q_h : 0);
           for (int c = lane; c < kD / 8; c += 32)
             cp_async16_or_zero(sbase + PL::kOffQ + (uint32_t)(c >> 3) * PL::kQChunk + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? 16 * c : 0), in);
@@ -608,7 +597,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     // The block two ahead of the one requested is brought into L2: the load that follows a freed slot then takes L2's latency.
     const int count = ms.count;
     Ahead<false> next(ms, p, 0, kBlock, lane);
-    Turn mine_to_bring{p.row_tiles, rt};
     const uint64_t pol = l2_policy_evict_first();
     const uint32_t mine = sbase + PL::kOffKV + lane * kChunkBytes;
     int asked = 0;
@@ -625,10 +613,8 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
           tma_load_3d_hint(mine + (kb & 1) * kSlotBytes, &map_kv, 64 * lane, row, page, &ms.kv_full[kb & 1][j], pol);
         asked = kGroups * kb + j + 1;
       }
-      if (mine_to_bring()) {
-        const uint8_t* src = next.rows_of(p, 2, 2 * kD);
-        if (src != nullptr && lane == 0) l2_prefetch_1d(src, kBlock * 2 * kD);
-      }
+      const uint8_t* src = next.rows_of(p, 2, 2 * kD);
+      if (src != nullptr && lane == 0) l2_prefetch_1d(src, kBlock * 2 * kD);
     }
     if (!ok)                                                              // given up: what is in flight lands first
       for (int i = max(asked - kSlots * kGroups, 0); i < asked; ++i) {
@@ -664,7 +650,6 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
       if (++at == w.k1) piece();
       return x;
     };
-    Turn mine_to_bring{p.row_tiles, rt};
     auto rows_of = [&](const Coming& x) -> const uint8_t* {
       return (unsigned)x.page < (unsigned)p.n_blocks ? p.cache + (long long)x.page * p.block_pitch + (long long)x.row * kRowBytes : nullptr;
     };
@@ -681,7 +666,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         c0 = c1; c1 = c2; c2 = c3; c3 = look();
         const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
         const uint8_t* src = rows_of(c0);
-        if (mine_to_bring()) to_l2(c2);
+        to_l2(c2);
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) {
           if (kb >= kSlots && !(ok = __all_sync(0xffffffffu, mbar_wait(&ms.kv_free[kb & 1][j], ((kb >> 1) & 1) ^ 1, wt, kSiteFree, kb)))) break;
@@ -726,7 +711,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
         c0 = c1; c1 = c2; c2 = c3; c3 = look();
         const uint32_t slot = sbase + PL::kOffKV + (kb & 1) * kSlotBytes;
         const uint8_t* next = rows_of(c1);
-        if (mine_to_bring()) to_l2(c2);
+        to_l2(c2);
         float4 mult[kSets];
 #pragma unroll
         for (int i = 0; i < kSets; ++i) mult[i] = scale[i];
@@ -762,7 +747,7 @@ mla_decode_kernel(const __grid_constant__ CUtensorMap map_kv, const __grid_const
     }
   }
 
-  if (warp == kWarpQk && rt == 0 && lane == 0 && p.meta) write_meta(p, ms, g);
+  if (warp == kWarpQk && lane == 0 && p.meta) write_meta(p, ms, g);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -943,7 +928,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps, 2) mla_decode_merge_kernel(c
 template <int kRows, Load kLoad>
 static int launch(const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {
   if (!ensure_smem<mla_decode_kernel<kRows, kLoad>>(current_device(), Plan<kRows>::kSmem)) return LITEDSA_ERR_CUDA;
-  return launch_pdl(mla_decode_kernel<kRows, kLoad>, dim3((unsigned)(p.groups * p.row_tiles)), kThreads<kLoad>, Plan<kRows>::kSmem, st, map, map_q, p);
+  return launch_pdl(mla_decode_kernel<kRows, kLoad>, dim3((unsigned)p.groups), kThreads<kLoad>, Plan<kRows>::kSmem, st, map, map_q, p);
 }
 template <int kRows>
 static int launch(Load l, const CUtensorMap& map, const CUtensorMap& map_q, const Params& p, cudaStream_t st) {

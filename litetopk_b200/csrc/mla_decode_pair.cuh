@@ -147,6 +147,15 @@ __device__ __forceinline__ void mma2_pair(uint32_t d, uint32_t a_lo, uint32_t a_
       ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate_first), "n"(kDa), "n"(kDb) : "memory");
 }
 
+// What a group's pairs bring into L2 they bring in turn: true once in `every` calls, the first time after `left` of them
+struct Turn {
+  int every, left;
+  __device__ __forceinline__ bool operator()() {
+    if (left-- > 0) return false;
+    left = every - 1;
+    return true;
+  }
+};
 // a running block's slot and the parity of its barriers
 template <int kSlots>
 struct Ring {
