@@ -462,7 +462,7 @@ int litedsa_index_status(int* out4_host, int reset);
  *             blocks block_stride_bytes apart (a multiple of 16), rows dense
  *   interleaved: pairs (2i, 2i + 1) of dims are turned, else pairs (i, i + 32)
  *   q_rope    [T, heads, 64] bf16 -> q_out, turned the same way (may be the same memory), or both NULL
- *   k_out     [T, 64] bf16: the turned k_rope once more, or NULL
+ *   k_out     [T, 64] bf16: the turned k_rope once more, or NULL.  Neither q_out nor k_out overlaps itself (strides of 0, say)
  * A packed group's scale is the smallest power of two that brings its 128 dims into +-448 (at least 2^-126).  A token whose
  * slot is negative or beyond the cache has no row written (padding); one whose position is not in the table is left out altogether.
  */

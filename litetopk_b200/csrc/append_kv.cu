@@ -149,6 +149,15 @@ __global__ void __launch_bounds__(32 * (kMaxHeadWarps + 1)) append_kv_kernel(con
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(row + 512 + (lane >> 1)) = (uint32_t)(e + 127) << 23;
 }
 
+// whether vectors of 64 elements in two dimensions lie apart
+static bool apart(int64_t n0, int64_t stride0, int64_t n1, int64_t stride1) {
+  if (n0 <= 1) return n1 <= 1 || stride1 >= 64;
+  if (n1 <= 1) return stride0 >= 64;
+  const bool inner1 = stride1 <= stride0;
+  const int64_t in = inner1 ? stride1 : stride0, out = inner1 ? stride0 : stride1, n = inner1 ? n1 : n0;
+  return in >= 64 && (out - 64) / in >= n - 1;
+}
+
 }  // namespace append
 }  // namespace lt
 
@@ -169,6 +178,9 @@ extern "C" int litedsa_append_kv(const void* kv_c, int64_t kv_c_stride, const vo
     return LITEDSA_ERR_UNSUPPORTED;
   if ((kv_c_stride | k_rope_stride | (q_rope ? q_token_stride | q_head_stride | q_out_token_stride | q_out_head_stride : 0) |
        (k_out ? k_out_stride : 0)) % 8 || cos_sin_stride % 4 || block_stride_bytes % 16)
+    return LITEDSA_ERR_UNSUPPORTED;
+  // (several threads would write the same words)
+  if ((q_rope && !append::apart(T, q_out_token_stride, heads, q_out_head_stride)) || (k_out && !append::apart(T, k_out_stride, 1, 0)))
     return LITEDSA_ERR_UNSUPPORTED;
   if (T == 0) return LITEDSA_OK;
   append::Params p = {};

@@ -239,6 +239,17 @@ PyObject* lite_topk(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// whether vectors of 64 elements in the dimensions before the last lie apart
+bool apart(const Tensor& t) {
+  int64_t n[2] = {1, 1}, stride[2] = {64, 64}, used = 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1) {
+      n[used] = t.size(i);
+      stride[used++] = t.stride(i);
+    }
+  const int64_t inner = stride[0] <= stride[1] ? 0 : 1;
+  return stride[inner] >= 64 && (used < 2 || (stride[1 - inner] - 64) / stride[inner] >= n[inner] - 1);
+}
 bool is_index(const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
 // A paged cache as dense.py takes it: [blocks, block_size, 576] bf16 or [blocks, block_size, 656] bytes, rows of a block dense
 bool paged(const Tensor& t, bool* packed, int64_t* pitch) {
@@ -269,7 +280,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return t.dim() == 2 && t.scalar_type() == at::kBFloat16 && t.size(0) == T && t.size(1) == d && t.stride(1) == 1;
     };
     auto index = [&](const Tensor& t) { return is_index(t) && t.dim() == 1 && t.size(0) == T && t.is_contiguous(); };
-    if (c->dim() != 2 || T <= 0 || !small(T) || !rows(*c, 512) || !rows(*k, 64) || (ko && !rows(*ko, 64)) || !index(*pos) || !index(*slots) ||
+    if (c->dim() != 2 || T <= 0 || !small(T) || !rows(*c, 512) || !rows(*k, 64) || (ko && (!rows(*ko, 64) || !apart(*ko))) || !index(*pos) || !index(*slots) ||
         cs->dim() != 2 || cs->scalar_type() != at::kFloat || cs->size(1) != 64 || cs->stride(1) != 1 || cs->size(0) <= 0)
       Py_RETURN_NONE;
     int64_t heads = 0;
@@ -278,7 +289,7 @@ PyObject* append_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return t.dim() == 3 && t.scalar_type() == at::kBFloat16 && t.size(0) == T && t.size(1) == heads && t.size(2) == 64 && t.stride(2) == 1;
       };
       heads = q->dim() == 3 ? q->size(1) : 0;
-      if (heads <= 0 || !small(heads) || !turned(*q) || !turned(*qo)) Py_RETURN_NONE;
+      if (heads <= 0 || !small(heads) || !turned(*q) || !turned(*qo) || !apart(*qo)) Py_RETURN_NONE;
     }
     int rc;
     {

@@ -44,6 +44,15 @@ def _cache(kv_cache: torch.Tensor):
     return packed, kv_cache.shape[0], kv_cache.shape[1], kv_cache.stride(0) * item
 
 
+def _apart(t: torch.Tensor, name: str) -> None:
+    steps = sorted((step, size) for step, size in zip(t.stride()[:-1], t.shape[:-1]) if size > 1)
+    end = t.shape[-1]
+    for step, size in steps:
+        if step < end:
+            raise ValueError(f"{name} must not overlap itself")
+        end += step * (size - 1)
+
+
 def append_kv(kv_c: torch.Tensor, k_rope: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, slots: torch.Tensor,
               kv_cache: torch.Tensor, *, interleaved: bool = True, q_rope: Optional[torch.Tensor] = None,
               q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> None:
@@ -57,7 +66,7 @@ def append_kv(kv_c: torch.Tensor, k_rope: torch.Tensor, positions: torch.Tensor,
 
     ``interleaved``: dims (2i, 2i + 1) are a pair, else (i, i + 32).  ``q_rope`` [T, heads, 64] bf16 is turned into
     ``q_out`` of that shape (any views with unit inner stride: the last 64 dims of projected and of absorbed queries; the same
-    view for in place), ``k_rope`` once more into ``k_out`` [T, 64] where that is given.
+    view for in place), ``k_rope`` once more into ``k_out`` [T, 64] where that is given.  Neither may overlap itself.
 
     Tokens with a slot that is negative or beyond the cache are padding: no row is written for them.  No two tokens may have the same
     slot.  Tokens whose position is not in ``cos_sin`` are left out altogether.
@@ -89,11 +98,13 @@ def append_kv(kv_c: torch.Tensor, k_rope: torch.Tensor, positions: torch.Tensor,
         heads = q_rope.shape[1]
         if q_rope.shape != (T, heads, 64) or q_out.shape != q_rope.shape or q_rope.stride(2) != 1 or q_out.stride(2) != 1 or heads < 1:
             raise ValueError("q_rope and q_out must be [T, heads, 64] with unit inner stride")
+        _apart(q_out, "q_out")
         qs, qo = q_rope.stride()[:2], q_out.stride()[:2]
     if k_out is not None:
         _need(k_out, "k_out", torch.bfloat16, 2)
         if k_out.shape != (T, 64) or k_out.stride(1) != 1:
             raise ValueError("k_out must be [T, 64] with unit inner stride")
+        _apart(k_out, "k_out")
     _same_device(dev, k_rope=k_rope, positions=positions, cos_sin=cos_sin, slots=slots, kv_cache=kv_cache, q_rope=q_rope, q_out=q_out, k_out=k_out)
     if T == 0:
         return
