@@ -38,10 +38,6 @@ __device__ __forceinline__ long long index_at(const void* p, int wide, int i) {
 __device__ __forceinline__ uint4 load16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ float lo_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 
 // A vector of 64 dims has eight lanes, 16 bytes each: four pairs of neighbours, or eight dims whose partners lane j ^ 4 has.
 template <bool kInterleaved>

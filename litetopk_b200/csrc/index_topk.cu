@@ -84,11 +84,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 __device__ int g_status[8];
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-  return e != 0;
-}
 
 // accs: accumulators in use, a CTA's tokens are accs * 128 / HI (a run-time number costs spills)
 template <int HI, int accs>

@@ -171,11 +171,6 @@ struct Item {
 __device__ __forceinline__ uint32_t low_bits(int x) {
   return x <= 0 ? 0u : (x >= 32 ? 0xffffffffu : ((1u << x) - 1u));
 }
-__device__ __forceinline__ bool elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-  return e != 0;
-}
 __device__ __forceinline__ void commit_one(uint32_t a) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(a) : "memory");
 }
