@@ -504,7 +504,7 @@ int litedsa_mla_decode_status(int* out4_host, int reset);
  *   q       [Tq, heads, 192] bf16, k_nope [Tk, heads, 128] bf16, k_rope [Tk, 64] bf16 (one for all heads), v [Tk, heads, 128] bf16
  *           (strides in elements, multiples of 8 and not 0; bases 16-byte aligned)
  *   cu_q, cu_k  [B + 1] int32: sequence b has queries [cu_q[b], cu_q[b + 1]) and keys [cu_k[b], cu_k[b + 1]); both NULL
- *           with B = 1: one sequence of all.  Entries are clamped to [0, Tq] and [0, Tk]; rows of out and lse that are no sequence's stay as they were
+ *           with B = 1: one sequence of all.  Entries do not fall, and are clamped to [0, Tq] and [0, Tk]; rows of out and lse that are no sequence's stay as they were
  *   causal  query i of a sequence with n queries and m keys sees keys [0, m - n + 1 + i) (its queries are its last tokens), else all
  *   out     [Tq, heads, 128] bf16, lse [Tq, heads] fp32, dense
  *   workspace   litedsa_mla_prefill_workspace(Tq, Tk, heads) bytes (0 for most sizes) on the current device, 16-byte

@@ -21,9 +21,10 @@
 // Packed rows (512 e4m3 codes, four fp32 scales, 64 bf16) pass through registers: sixteen warps load a block ahead, convert it to
 // bf16 (exact where the scales are powers of two) and write the same tile that TMA writes for bf16 rows.
 //
-// Bound by memory up to 16 rows, by the tensor cores from 64 on.  Measured: 5 sequences of 65 to 131 thousand keys, 16 heads, bf16, 103 us = 5.5 TB/s
-// with the merge (a copy: 6.5); 32 sequences of up to 8191 packed keys, 64 heads, 52 us, where fifteen blocks a CTA take 3800 cycles each, the
-// latency of loads, conversion, products and softmax over two slots, and start, pieces' ends and merge 20 us.
+// Bound by memory up to 16 rows, by the tensor cores from 64 on.  Measured: 5 sequences of 65 to 131 thousand keys, 16 heads, bf16, 113 us = 5.0 TB/s
+// with the merge (a copy: 6.5), 103 in the first calls; 64 heads 127, 113 in the first calls; 32 sequences of up to 8191 packed keys, 64 heads, 51 us,
+// where fifteen blocks a CTA take 3800 cycles each, the latency of loads, conversion, products and softmax over two slots, and start, pieces' ends and
+// merge 20 us.
 //
 // A key beyond the sequence's end is in no product: its S is replaced, and its value row is zeroed before the second product, whatever its page holds.
 // A row's sum of exponentials is 0 where it sees no key, and NaN where a score is NaN or +infinity: maxima pass NaN over, sums and products keep it, and the
@@ -42,8 +43,10 @@ constexpr uint32_t kSlotBytes = kChunks * kChunkBytes;
 constexpr int kSlots = 2;
 constexpr int kMostStartCost = 5;                           // blocks
 constexpr int kGroups = 5;                                  // a tile's chunks are loaded and given back in groups: four of 128 dims, the rope dims
-// Warps 0-7: softmax.  Who loads: one warp by TMA (bf16 rows in pages of multiples of 64), 8 by cp.async (bf16 rows in smaller pages:
-// a box is a page then, and 36 boxes a block take a warp 3400 cycles to issue), 16 through registers (packed rows).
+// Warps 0-7: softmax.  Who loads: one warp by TMA (bf16 rows in pages of multiples of 64), 8 by cp.async (bf16 rows in other pages:
+// a box is 16 rows then, and 36 boxes a block take a warp 3400 cycles to issue), 16 through registers (packed rows).  TMA / cp.async with pages of 64, us:
+// 5 sequences of 65 to 131 thousand keys, 64 heads 127 / 132, 16 heads 113 / 116; 32 of up to 8191, 64 heads, 47 / 52; 64 of 1000 to 4000, 32 heads, 48 / 52.
+// cp.async takes as long with pages of 16.
 enum Load { kTma, kCopy, kPacked };
 constexpr int kSoftmaxWarps = 8, kWarpQk = 8, kWarpPv = 9, kWarpQ = 10, kWarpTma = 11, kWarpLoad0 = 12;
 template <Load kLoad> constexpr int kLoadWarps = kLoad == kTma ? 0 : kLoad == kCopy ? 8 : 16;
@@ -992,7 +995,10 @@ extern "C" int litedsa_mla_decode(const void* q, int64_t q_batch_stride, int64_t
   p.B = B; p.q_len = q_len; p.heads = heads; p.rows = q_len * heads; p.row_tiles = s.tiles; p.groups = s.groups;
   p.cols = n_blocks == 0 ? 0 : table_cols; p.block_size = block_size; p.n_blocks = (int)n_blocks;
   // 7000 cycles at 1400 to 2600 a block of a pair, 5500 at 3000 to 3800 of a CTA (0 / 2 / 4 / 6: 256 rows, bf16 109 / 106 / 103 / 102 us; 128 rows, packed 147 /
-  // 142 / 144 / 146; 64 rows, packed 57.7 / 52.0 / 51.9 / 53.4; 16 rows, packed 44.9 / 44.4 / 46.4 / 48.9)
+  // 142 / 144 / 146; 64 rows, packed 57.7 / 52.0 / 51.9 / 53.4; 16 rows, packed 44.9 / 44.4 / 46.4 / 48.9).  Elsewhere, 0 / 2 / 5 / 8, between two events behind a
+  // flush of L2: 16 heads, 20 x 500-3000 keys, bf16 30 / 28 / 28 / 28; 64 heads, 10 x 5000-30000, bf16 64 / 62 / 62 / 62; 32 heads, 64 x 100-3000, packed
+  // 50 / 46 / 48 / 50; 64 heads, 300 x 64-600, packed 67 / 62 / 62 / 62; 128 heads, bf16, 20 x 2000-20000 87 / 86 / 85 / 85, 200 x 100-900 75 / 69 / 65 / 67;
+  // 128 heads, 300 x 100-900, packed 99 / 95 / 91 / 93; three tokens of 128 heads, 40 x 500-3000, packed 101 / 97 / 95 / 99
   p.start_cost = s.pair && !packed ? kMostStartCost : 2;
   p.box_rows = block_size % pair::kOwnKeys == 0 ? pair::kOwnKeys : 16;
   p.scale_log2 = sm_scale * kLog2e;

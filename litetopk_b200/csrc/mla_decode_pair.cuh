@@ -15,9 +15,10 @@
 // (mla_prefill.cu).  A CTA whose rows need one has four warps of the other do their part and holds its P back until that is
 // done; asking each other every block took 1600 cycles of it.
 //
-// Measured: 48 sequences of 1000 to 6001 keys, two tokens of 128 heads, bf16 in pages of 16, 100.5 us (one CTA to 64 rows: 133): a block a pair takes 1400 cycles,
-// the tensor pipe is at 74 %; change of sequence 7000 cycles.  128 sequences of 2048 to 4096 packed keys, 128 heads, 139.5 us (215): 2600 cycles, which are
-// the converting warps' instructions (their loads wait for nothing; the tensor pipe is at 57 %, the issue slots at 61 %).
+// Measured: 48 sequences of 1000 to 6001 keys, two tokens of 128 heads, bf16 in pages of 16, 100.5 us in a few calls (one CTA to 64 rows: 133), 120 at the
+// power limit: a block a pair takes 1400 cycles, the tensor pipe is at 74 %; change of sequence 7000 cycles.  128 sequences of 2048 to 4096 packed keys, 128
+// heads, 139.5 us (215), 165 at the power limit: 2600 cycles, which are the converting warps' instructions (their loads wait for nothing; the tensor pipe is at
+// 57 %, the issue slots at 61 %).
 #pragma once
 
 namespace lt {

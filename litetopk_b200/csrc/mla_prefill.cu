@@ -19,9 +19,10 @@
 // tiles first, heads one after the other so that the CTAs that run share their K and V in L2.  A call of few tiles leaves
 // most of its last wave idle: its last tiles are cut along the keys, and a second kernel merges the pieces in fp32.
 //
-// Measured: 8192 tokens x 64 heads, causal, 1047 us = 1312 TFLOP/s in a few calls, 1217 us = 1129 TFLOP/s when the power limit has brought the clock down
-// to 1.55 GHz (a library's matrix product: 1657 and 1391); 4096 tokens behind 28672, 16 heads, 957 us = 1346 TFLOP/s.  A block of a tile takes 2000
-// cycles of a CTA, of which the tensor cores compute 1300: the exponentials (128 a row and block) and the hand-overs fill the rest.
+// Measured: 8192 tokens x 64 heads, causal, 1221 us = 1126 TFLOP/s when the power limit has brought the clock down to 1.55 GHz, 1047 = 1312 in a few calls
+// (a library's matrix product: 1391 and 1657); 4096 tokens behind 28672, 16 heads, 1107 us = 1164 TFLOP/s, 957 = 1346 in a few calls.  A block of a tile takes
+// 2000 cycles of a CTA, of which the tensor cores compute 1300: the exponentials (128 a row and block) and the hand-overs fill the rest.  Works of up to 128
+// queries have one tile at work and nothing beside it: 4 tokens behind 16384, 64 heads, 147 us (their bytes: 82).
 #include "common.cuh"
 #include "tensor_map.cuh"
 
@@ -129,7 +130,9 @@ __device__ __forceinline__ Cut cut_of(int tiles, int most_blocks, const Params& 
 }
 
 // Calls of many tiles take those of more than a third of the longest one's blocks first, of all heads, then the others: what the last CTAs to
-// finish are still at is then short (a batch of 11 sequences 398 -> 376 us, 8192 tokens of 64 heads 1101 -> 1047).  Among the first and among the others, as in
+// finish are still at is then short (a batch of 11 sequences 398 -> 376 us, 8192 tokens of 64 heads 1101 -> 1047, all in a few calls; in one order / from a
+// quarter / a third / half on, between two events behind a flush of L2, us: 5 prompts of 100 to 6000 tokens, 32 heads, 723 / 693 / 708 / 689, 40 of 50 to 900, 16 heads, 135 / 132 / 121 / 133, 3 of 4000,
+// 24 heads, 372 / 357 / 349 / 350; but 20 of 300 to 700 behind 2000, 16 heads, 271 / 280 / 280 / 282, where all tiles are among the first and the order is one).  Among the first and among the others, as in
 // calls of few: a head's tiles from its last to its first, then the next head's, so that CTAs that run together share keys and values in L2.
 //
 // A lane keeps how many tiles the sequences [0, (lane + 1) each) have among the first and among the others, and of `each` = 1 its sequence: to find a

@@ -183,7 +183,7 @@ def mla_prefill(q: torch.Tensor, k_nope: torch.Tensor, k_rope: torch.Tensor, v: 
 
     q [Tq, heads, 192], k_nope and v [Tk, heads, 128], k_rope [Tk, 64] (one for all heads), all bf16; any strides but 0 that are multiples
     of 8, unit inner stride (k_nope and v may be views of one projection).  Sequence b has queries ``cu_seqlens_q[b] : cu_seqlens_q[b + 1]`` and
-    keys ``cu_seqlens_k[b] : cu_seqlens_k[b + 1]`` (int32 [B + 1]; both None: one sequence of all).  ``causal``: its queries are its last tokens,
+    keys ``cu_seqlens_k[b] : cu_seqlens_k[b + 1]`` (int32 [B + 1], entries that do not fall; both None: one sequence of all).  ``causal``: its queries are its last tokens,
     query i of n sees the first ``m - n + 1 + i`` of its m keys.  ``sm_scale`` must not be negative.
 
     Returns ``(out [Tq, heads, 128] bf16, lse [Tq, heads] f32)``, written into ``out`` / ``lse`` when given (contiguous).  A row that sees
