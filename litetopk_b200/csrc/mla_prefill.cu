@@ -131,9 +131,10 @@ __device__ __forceinline__ Cut cut_of(int tiles, int most_blocks, const Params& 
 
 // Calls of many tiles take those of more than a third of the longest one's blocks first, of all heads, then the others: what the last CTAs to
 // finish are still at is then short (a batch of 11 sequences 398 -> 376 us, 8192 tokens of 64 heads 1101 -> 1047, all in a few calls; in one order / from a
-// quarter / a third / half on, between two events behind a flush of L2, us: 5 prompts of 100 to 6000 tokens, 32 heads, 723 / 693 / 708 / 689, 40 of 50 to 900, 16 heads, 135 / 132 / 121 / 133, 3 of 4000,
-// 24 heads, 372 / 357 / 349 / 350; but 20 of 300 to 700 behind 2000, 16 heads, 271 / 280 / 280 / 282, where all tiles are among the first and the order is one).  Among the first and among the others, as in
-// calls of few: a head's tiles from its last to its first, then the next head's, so that CTAs that run together share keys and values in L2.
+// quarter / a third / half on, between two events behind a flush of L2, us: 5 prompts of 100 to 6000 tokens, 32 heads, 723 / 693 / 708 / 689, 40 of 50 to 900,
+// 16 heads, 135 / 132 / 121 / 133, 3 of 4000, 24 heads, 372 / 357 / 349 / 350; but 20 of 300 to 700 behind 2000, 16 heads, 271 / 280 / 280 / 282, where all
+// tiles are among the first and the order is one).  Among the first and among the others, as in calls of few: a head's tiles from its last to its first, then
+// the next head's, so that CTAs that run together share keys and values in L2.
 //
 // A lane keeps how many tiles the sequences [0, (lane + 1) each) have among the first and among the others, and of `each` = 1 its sequence: to find a
 // work's tile then takes one read of memory where there are up to 1024 sequences, none up to 32.  (Looking 32 sequences at a time through all of them, 1000
